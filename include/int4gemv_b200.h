@@ -300,6 +300,103 @@ int int4gemv_w4a16_exchange_static(void* y, const void* x, const void* qweight,
                                    const void* scales, const void* zeros, int64_t m, int64_t n,
                                    int64_t k, int64_t group_size, int mode, void* stream);
 
+/* ---- Decode-step operators around the GEMV (new: the reference has only the GEMV) ------------- */
+
+/* What a decode step needs between its matrix products: the norm before a projection, the
+ * attention over a paged cache and the cache's eviction, and the log probabilities behind the last
+ * one. They are launched like the pipelined GEMVs (programmatic stream serialization), but read
+ * nothing before the previous kernel in the stream has completed. */
+
+/* Root-mean-square norm with the residual's addition. Per row of x [rows, hidden]:
+ *   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight,
+ * computed in fp32 from the unrounded sum; h and y are rounded once. x, residual, weight [hidden],
+ * h and y have one element type, dtype (INT4GEMV_DTYPE_F32, _F16 or _BF16). residual may be NULL (h = x);
+ * h may then be NULL too, and is not written. h may be x or residual itself. Any hidden >= 1;
+ * fastest when all pointers are 16-byte aligned. */
+int int4gemv_add_rms_norm(void* y, void* h, const void* x, const void* residual, const void* weight,
+                          float eps, int dtype, int64_t rows, int64_t hidden, void* stream);
+
+/* The same with y in 8 bits: scales[row] = max(max|y| / 448, 1e-12) (fp32), y = the e4m3 value
+ * nearest to y / scales[row]. A row with a NaN or infinite sum has a NaN scale. */
+int int4gemv_add_rms_norm_quant(void* y, float* scales, void* h, const void* x, const void* residual,
+                                const void* weight, float eps, int dtype, int64_t rows,
+                                int64_t hidden, void* stream);
+
+/* A paged cache. k and v hold [num_blocks, block_size, kv_heads, head_dim] elements (fp16 or bf16)
+ * with any strides of the first three dimensions that are multiples of 8 elements (so head-major
+ * pages, and k and v as two halves of one tensor, need no copy); the head_dim elements of a head
+ * are contiguous, head_dim a multiple of 8 up to INT4GEMV_MAX_HEAD_DIM; k and v 16-byte aligned.
+ * weights [num_blocks, kv_heads, block_size] fp32, contiguous: the attention weight every position
+ * has received so far (NULL where it is not used). Position j of sequence b stands in page
+ * block_table[b][j / block_size] at offset j % block_size. */
+#define INT4GEMV_MAX_HEAD_DIM 256
+typedef struct {
+  void* k;
+  void* v;
+  float* weights;
+  int64_t num_blocks, block_size, kv_heads, head_dim;
+  int64_t k_strides[3], v_strides[3]; /* block, position in the block, head */
+  int32_t dtype;                      /* INT4GEMV_DTYPE_F16 or _BF16 */
+  int32_t reserved;
+} int4gemv_paged_cache_t;
+
+/* sizeof(int4gemv_paged_cache_t), for bindings that build the struct themselves. */
+size_t int4gemv_paged_cache_struct_bytes(void);
+
+/* Attention of one new token a sequence: out [batch, q_heads, head_dim] =
+ * softmax(scale q k^T) v over positions [0, seq_lens[b]) of sequence b, query head h reading KV
+ * head h / (q_heads / kv_heads); q and out have the cache's type, the softmax and the sums are fp32.
+ * A sequence of length 0 gives zeros. block_table [batch, max_blocks] and seq_lens [batch] are
+ * int32; table entries behind a sequence's last page are not read.
+ * k_new, v_new ([batch, kv_heads, head_dim], or both NULL): the new token's key and value. seq_lens
+ * counts that token; they are written to the slot of position seq_lens[b] - 1 and used for it.
+ * That slot must not belong to another sequence of the batch.
+ * add_weights: weights[page, g, offset] += the sum of the probabilities of the query heads of KV
+ * head g, at every position; with k_new the new token's slot is set, not added to. Sequences of
+ * one batch that share a page must then be given in different calls.
+ * A length outside of [0, max_blocks block_size] is clamped, a page outside of [0, num_blocks) is
+ * left out, and int4gemv_device_status reports 4; nothing outside of the cache is touched.
+ * workspace: int4gemv_paged_attention_workspace_size bytes on the device, 256-byte aligned, used
+ * within the call in stream order (calls that may overlap need one each); its content does not
+ * matter. The result does not depend on timing. */
+int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cache_t* cache,
+                             const int32_t* block_table, const int32_t* seq_lens, float scale,
+                             const void* k_new, const void* v_new, int add_weights, int64_t batch,
+                             int64_t q_heads, int64_t max_blocks, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace for the current device, or -1 if the sizes are refused (see
+ * int4gemv_last_error). The pointers of `cache` are not used. */
+int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* cache, int64_t batch,
+                                                int64_t q_heads, int64_t max_blocks, int weights);
+
+/* Eviction by accumulated attention weight. For every sequence and KV head, of its
+ * n = seq_lens[b] positions the last `recent` stay and, of the others, the budget - recent with
+ * the largest weights (of equal ones the lowest position; a NaN counts as largest); all of them
+ * where n <= budget. The keys, values and weights of what stays are copied, in their old order, to
+ * positions 0, 1, ... of the pages in new_table [batch, new_blocks]; new_lens [batch] =
+ * min(n, budget); kept [batch, kv_heads, budget] holds the old positions, then -1. Heads choose
+ * for themselves: afterwards position j of two heads may come from different tokens. The new pages
+ * must not be among the old ones, nor be named twice; the old pages are left as they were, so
+ * sequences may share them. Lengths and pages outside of the cache are treated as in
+ * int4gemv_paged_attention (an unreadable weight counts as lowest, an unreadable page is not copied). */
+int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_cache_t* cache,
+                         const int32_t* block_table, const int32_t* seq_lens,
+                         const int32_t* new_table, int64_t budget, int64_t recent, int64_t batch,
+                         int64_t max_blocks, int64_t new_blocks, void* stream);
+
+/* Per row x of logits [rows, vocab] (fp32, fp16 or bf16, rows row_stride elements apart):
+ * logprobs = x[tokens] - lse with lse = log sum e^x, entropy = lse - sum softmax(x) x, and the
+ * `top` largest log probabilities with their indices, largest first, the lowest index first among
+ * equal ones. All sums and results are fp32, indices int64. A token outside of [0, vocab) gives
+ * NaN. Logits of -inf have probability 0; a row with a NaN or +inf, or with nothing above -inf,
+ * gives NaN (its top_ids are the order of its logits, NaN first). top <= INT4GEMV_MAX_TOP and
+ * vocab; with top = 0 top_logprobs and top_ids are not used. */
+#define INT4GEMV_MAX_TOP 32
+int int4gemv_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                            const void* logits, const int64_t* tokens, int dtype, int64_t rows,
+                            int64_t vocab, int64_t row_stride, int64_t top, void* stream);
+
 /* ---- Stream ordering of the weights ---------------------------------------------------------- */
 
 /* The pipelined kernels (stripe_mma, tc_dequant, stream_mma, tcgen05, and the fused epilogues and
@@ -321,8 +418,9 @@ int int4gemv_set_strict_weights(int strict);
 
 /* Reads and clears the current device's kernel status word: 0 if every pipelined kernel since the
  * last call finished normally, else a nonzero code recorded by a kernel whose bounded wait on a
- * shared-memory barrier timed out (the kernel then skipped its work and returned). Synchronises
- * the current device. */
+ * shared-memory barrier timed out (the kernel then skipped its work and returned), or 4 by an
+ * operator on a paged cache that was given a length or page outside of it. Synchronises the
+ * current device. */
 int int4gemv_device_status(int* status);
 
 #ifdef __cplusplus

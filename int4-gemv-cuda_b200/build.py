@@ -38,10 +38,11 @@ CU_SOURCES = [
     "tc_dequant.cu", "tc_wide.cu",
     "weight_stream.cu",
     "packed.cu", "quantize.cu", "repack.cu",
+    "add_rms_norm.cu", "paged_attention.cu", "paged_evict.cu", "token_logprobs.cu",
 ]
 # The CPU path must keep one IEEE rounding per operation: no contraction, no fast-math.
 CPU_SOURCES = {"sequential.cpp": ["-O3", "-ffp-contract=off", "-fno-fast-math"]}
-TORCH_SOURCES = ["bindings.cpp", "checks.cpp"]
+TORCH_SOURCES = ["bindings.cpp", "checks.cpp", "decode_ops.cpp"]
 HEADERS = list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [INCLUDE / "int4gemv_b200.h"]
 
 

@@ -391,6 +391,18 @@ PYBIND11_MODULE(int4gemv_ops, m) {
   m.def("repack_gptq", &int4gemv::repack_gptq, py::arg("qweight"), py::arg("qzeros"),
         py::arg("scales"), py::arg("group_size"), py::arg("zero_offset") = 1);
   m.def("pack", &int4gemv::pack, py::arg("q"));
+  m.def("add_rms_norm", &int4gemv::add_rms_norm, py::arg("x"), py::arg("weight"),
+        py::arg("eps") = 1e-5, py::arg("residual") = py::none());
+  m.def("add_rms_norm_quant", &int4gemv::add_rms_norm_quant, py::arg("x"), py::arg("weight"),
+        py::arg("eps") = 1e-5, py::arg("residual") = py::none());
+  m.def("paged_attention", &int4gemv::paged_attention, py::arg("q"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("block_table"), py::arg("seq_lens"), py::arg("scale"),
+        py::arg("k") = py::none(), py::arg("v") = py::none(), py::arg("weights") = py::none());
+  m.def("paged_evict", &int4gemv::paged_evict, py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("weights"), py::arg("block_table"), py::arg("seq_lens"), py::arg("new_table"),
+        py::arg("budget"), py::arg("recent"));
+  m.def("token_logprobs", &int4gemv::token_logprobs, py::arg("logits"), py::arg("tokens"),
+        py::arg("top") = 0);
   m.def(
       "check_inputs",
       [](const char* name, const at::Tensor& x, const at::Tensor& qweight,

@@ -238,11 +238,127 @@ int static_scratch(const char* name, void** out, void** counters) {
 }
 }  // namespace
 
+// ---- Checks of the decode-step operators ----------------------------------------------------------
+namespace {
+
+bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int check_dtype(const char* name, int dtype, bool f32) {
+  if (dtype == INT4GEMV_DTYPE_F16 || dtype == INT4GEMV_DTYPE_BF16 || (f32 && dtype == INT4GEMV_DTYPE_F32)) {
+    return INT4GEMV_OK;
+  }
+  return fail(INT4GEMV_ERR_INVALID, "%s: unsupported dtype %d", name, dtype);
+}
+
+int run_norm(const char* name, i4::NormArgs a, int dtype, int64_t rows, int64_t hidden,
+             cudaStream_t st) {
+  if (int e = check_dtype(name, dtype, true)) return e;
+  if (rows < 0 || hidden < 1 || rows > INT_MAX || hidden > INT_MAX / 2) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: rows = %lld, hidden = %lld are out of range", name,
+                static_cast<long long>(rows), static_cast<long long>(hidden));
+  }
+  if (rows == 0) return ok();
+  if (!a.x || !a.weight || !a.y) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  if (a.residual && !a.h) return fail(INT4GEMV_ERR_INVALID, "%s: a residual needs h", name);
+  const size_t size = dtype == INT4GEMV_DTYPE_F32 ? 4 : 2;
+  for (const void* p : {a.x, a.residual, a.weight, static_cast<const void*>(a.h)}) {
+    if (!aligned_to(p, size)) {
+      return fail(INT4GEMV_ERR_INVALID, "%s: x, residual, weight and h must be aligned to an element", name);
+    }
+  }
+  if (!aligned_to(a.y, a.scales ? 1 : size) || !aligned_to(a.scales, 4)) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: y and scales must be aligned to an element", name);
+  }
+  a.rows = static_cast<int>(rows);
+  a.hidden = static_cast<int>(hidden);
+  a.aligned = aligned_to(a.x, 16) && aligned_to(a.residual, 16) && aligned_to(a.weight, 16) &&
+              aligned_to(a.h, 16) && aligned_to(a.y, a.scales ? 16 / size : 16);
+  return launched(name, i4::launch_add_rms_norm(a, dtype, st));
+}
+
+// The checks that every operator on a paged cache makes of it.
+int check_cache(const char* name, const int4gemv_paged_cache_t* c) {
+  if (!c) return fail(INT4GEMV_ERR_INVALID, "%s: null cache", name);
+  if (int e = check_dtype(name, c->dtype, false)) return e;
+  if (c->head_dim < 8 || c->head_dim > INT4GEMV_MAX_HEAD_DIM || c->head_dim % 8 != 0) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: head_dim %lld must be a multiple of 8 in [8, %d]", name,
+                static_cast<long long>(c->head_dim), INT4GEMV_MAX_HEAD_DIM);
+  }
+  if (c->num_blocks < 0 || c->num_blocks > INT_MAX || c->block_size < 1 || c->block_size > INT_MAX ||
+      c->kv_heads < 1 || c->kv_heads > 65535) {
+    return fail(INT4GEMV_ERR_INVALID,
+                "%s: num_blocks = %lld, block_size = %lld, kv_heads = %lld are out of range", name,
+                static_cast<long long>(c->num_blocks), static_cast<long long>(c->block_size),
+                static_cast<long long>(c->kv_heads));
+  }
+  for (const int64_t* s : {c->k_strides, c->v_strides}) {
+    for (int i = 0; i < 3; ++i) {
+      if (s[i] < 0 || s[i] % 8 != 0) {
+        return fail(INT4GEMV_ERR_INVALID,
+                    "%s: the caches' strides must be non-negative multiples of 8 elements", name);
+      }
+    }
+  }
+  if (!aligned_to(c->k, 16) || !aligned_to(c->v, 16) || !aligned_to(c->weights, 4)) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: k and v must be 16-byte aligned, weights 4-byte", name);
+  }
+  return INT4GEMV_OK;
+}
+
+i4::PagedCache make_cache(const int4gemv_paged_cache_t* c, bool weights) {
+  return i4::PagedCache{c->k, c->v, c->k_strides[0], c->k_strides[1], c->k_strides[2],
+                        c->v_strides[0], c->v_strides[1], c->v_strides[2],
+                        weights ? c->weights : nullptr, static_cast<int>(c->num_blocks),
+                        static_cast<int>(c->block_size), static_cast<int>(c->kv_heads),
+                        static_cast<int>(c->head_dim)};
+}
+
+int check_batch(const char* name, int64_t batch, int64_t max_blocks) {
+  if (batch < 0 || batch > 65535 || max_blocks < 0 || max_blocks > INT_MAX) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: batch = %lld, max_blocks = %lld are out of range", name,
+                static_cast<long long>(batch), static_cast<long long>(max_blocks));
+  }
+  return INT4GEMV_OK;
+}
+
+// The sizes of a paged_attention call; `a` gets the cache and the counts.
+int attention_sizes(const char* name, const int4gemv_paged_cache_t* c, int64_t batch, int64_t q_heads,
+                    int64_t max_blocks, bool weights, i4::PagedAttentionArgs* a, int64_t* bytes) {
+  if (int e = check_cache(name, c)) return e;
+  if (int e = check_batch(name, batch, max_blocks)) return e;
+  if (q_heads < 1 || q_heads > 65535 || q_heads % c->kv_heads != 0) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: q_heads %lld must be a multiple of kv_heads %lld", name,
+                static_cast<long long>(q_heads), static_cast<long long>(c->kv_heads));
+  }
+  a->cache = make_cache(c, weights);
+  a->batch = static_cast<int>(batch);
+  a->hq = static_cast<int>(q_heads);
+  a->max_blocks = static_cast<int>(max_blocks);
+  *bytes = 0;
+  if (batch == 0) return INT4GEMV_OK;
+  // whether weights are asked for decides on the workspace: any non-null pointer will do here
+  static float any;
+  if (weights) a->cache.weights = &any;
+  *bytes = i4::paged_attention_workspace_bytes(*a);
+  if (*bytes == 0) {
+    return fail(INT4GEMV_ERR_INVALID,
+                "%s: batch = %lld with tables of %lld blocks of %lld is out of range", name,
+                static_cast<long long>(batch), static_cast<long long>(max_blocks),
+                static_cast<long long>(c->block_size));
+  }
+  a->cache.weights = weights ? c->weights : nullptr;
+  return INT4GEMV_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 const char* int4gemv_last_error(void) { return g_last_error.c_str(); }
 
-int int4gemv_version(void) { return 100; }
+int int4gemv_version(void) { return 200; }
 
 int int4gemv_naive(void* y, const void* x, const void* qweight, const void* scales,
                    const void* zeros, int64_t m, int64_t n, int64_t k, int64_t group_size,
@@ -855,6 +971,138 @@ int int4gemv_set_strict_weights(int strict) {
   }
   g_strict_weights.store(strict, std::memory_order_relaxed);
   return ok();
+}
+
+// ---- Decode-step operators ----------------------------------------------------------------------
+
+size_t int4gemv_paged_cache_struct_bytes(void) { return sizeof(int4gemv_paged_cache_t); }
+
+int int4gemv_add_rms_norm(void* y, void* h, const void* x, const void* residual, const void* weight,
+                          float eps, int dtype, int64_t rows, int64_t hidden, void* stream) {
+  i4::NormArgs a{x, residual, weight, h, y, nullptr, 0, 0, eps, false};
+  return run_norm("add_rms_norm", a, dtype, rows, hidden, static_cast<cudaStream_t>(stream));
+}
+
+int int4gemv_add_rms_norm_quant(void* y, float* scales, void* h, const void* x, const void* residual,
+                                const void* weight, float eps, int dtype, int64_t rows,
+                                int64_t hidden, void* stream) {
+  const char* name = "add_rms_norm_quant";
+  if (rows > 0 && !scales) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  i4::NormArgs a{x, residual, weight, h, y, scales, 0, 0, eps, false};
+  return run_norm(name, a, dtype, rows, hidden, static_cast<cudaStream_t>(stream));
+}
+
+int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* cache, int64_t batch,
+                                                int64_t q_heads, int64_t max_blocks, int weights) {
+  i4::PagedAttentionArgs a{};
+  int64_t bytes = 0;
+  if (attention_sizes("paged_attention", cache, batch, q_heads, max_blocks, weights != 0, &a, &bytes)) {
+    return -1;
+  }
+  return bytes;
+}
+
+int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cache_t* cache,
+                             const int32_t* block_table, const int32_t* seq_lens, float scale,
+                             const void* k_new, const void* v_new, int add_weights, int64_t batch,
+                             int64_t q_heads, int64_t max_blocks, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const char* name = "paged_attention";
+  i4::PagedAttentionArgs a{};
+  int64_t bytes = 0;
+  if (int e = attention_sizes(name, cache, batch, q_heads, max_blocks, add_weights != 0, &a, &bytes)) {
+    return e;
+  }
+  if (batch == 0) return ok();
+  const bool some_pages = a.cache.num_blocks > 0;
+  if (!out || !q || !seq_lens || (max_blocks > 0 && !block_table) ||
+      (some_pages && (!a.cache.k || !a.cache.v || (add_weights && !a.cache.weights)))) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  if (!k_new != !v_new) return fail(INT4GEMV_ERR_INVALID, "%s: k_new and v_new come together", name);
+  if (!aligned_to(q, 16) || !aligned_to(out, 16) || !aligned_to(k_new, 16) || !aligned_to(v_new, 16)) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: q, out, k_new and v_new must be 16-byte aligned", name);
+  }
+  if (!workspace || workspace_bytes < bytes || !aligned_to(workspace, 256)) {
+    return fail(INT4GEMV_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %lld bytes is needed, got %lld",
+                name, static_cast<long long>(bytes), static_cast<long long>(workspace ? workspace_bytes : 0));
+  }
+  // a flag for the kernel: weights are added where the pointer is set
+  if (add_weights && !some_pages) a.cache.weights = static_cast<float*>(workspace);
+  if (!some_pages) a.cache.k = a.cache.v = const_cast<void*>(q);  // an address that is not read
+  a.out = out;
+  a.q = q;
+  a.table = block_table;
+  a.lens = seq_lens;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.workspace = workspace;
+  return launched(name, i4::launch_paged_attention(a, cache->dtype, static_cast<cudaStream_t>(stream)));
+}
+
+int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_cache_t* cache,
+                         const int32_t* block_table, const int32_t* seq_lens,
+                         const int32_t* new_table, int64_t budget, int64_t recent, int64_t batch,
+                         int64_t max_blocks, int64_t new_blocks, void* stream) {
+  const char* name = "paged_evict";
+  if (int e = check_cache(name, cache)) return e;
+  if (int e = check_batch(name, batch, max_blocks)) return e;
+  if (int e = check_batch(name, batch, new_blocks)) return e;
+  if (budget < 1 || budget > INT_MAX || recent < 0 || recent > budget) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: budget %lld must be positive and recent %lld in [0, budget]",
+                name, static_cast<long long>(budget), static_cast<long long>(recent));
+  }
+  if (new_blocks * cache->block_size < budget) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: the new table has room for %lld positions, the budget is %lld",
+                name, static_cast<long long>(new_blocks * cache->block_size),
+                static_cast<long long>(budget));
+  }
+  if (max_blocks * cache->block_size > INT_MAX || batch * cache->kv_heads > INT_MAX ||
+      budget * cache->kv_heads / 8 > INT_MAX) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: batch = %lld with tables of %lld blocks of %lld is out of range",
+                name, static_cast<long long>(batch), static_cast<long long>(max_blocks),
+                static_cast<long long>(cache->block_size));
+  }
+  if (batch == 0) return ok();
+  const bool some_pages = cache->num_blocks > 0;
+  if (!kept || !new_lens || !seq_lens || (max_blocks > 0 && !block_table) || !new_table ||
+      (some_pages && (!cache->k || !cache->v || !cache->weights))) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  i4::PagedEvictArgs a{make_cache(cache, true), block_table, seq_lens, new_table, kept, new_lens,
+                       static_cast<int>(batch), static_cast<int>(max_blocks),
+                       static_cast<int>(new_blocks), static_cast<int>(budget),
+                       static_cast<int>(recent)};
+  return launched(name, i4::launch_paged_evict(a, static_cast<cudaStream_t>(stream)));
+}
+
+int int4gemv_token_logprobs(float* logprobs, float* entropy, float* top_logprobs, int64_t* top_ids,
+                            const void* logits, const int64_t* tokens, int dtype, int64_t rows,
+                            int64_t vocab, int64_t row_stride, int64_t top, void* stream) {
+  const char* name = "token_logprobs";
+  if (int e = check_dtype(name, dtype, true)) return e;
+  if (rows < 0 || vocab < 1 || rows > INT_MAX / 8 || vocab > (1 << 30) || row_stride < 0) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: rows = %lld, vocab = %lld, row_stride = %lld are out of range",
+                name, static_cast<long long>(rows), static_cast<long long>(vocab),
+                static_cast<long long>(row_stride));
+  }
+  if (top < 0 || top > INT4GEMV_MAX_TOP || top > vocab) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: top %lld must be in [0, %d] and at most vocab = %lld", name,
+                static_cast<long long>(top), INT4GEMV_MAX_TOP, static_cast<long long>(vocab));
+  }
+  if (rows == 0) return ok();
+  if (!logprobs || !entropy || !logits || !tokens || (top > 0 && (!top_logprobs || !top_ids))) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  if (!aligned_to(logits, dtype == INT4GEMV_DTYPE_F32 ? 4 : 2) || !aligned_to(tokens, 8)) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: logits and tokens must be aligned to an element", name);
+  }
+  i4::LogprobArgs a{logits, tokens, logprobs, entropy, top_logprobs, top_ids, row_stride,
+                    static_cast<int>(rows), static_cast<int>(vocab), static_cast<int>(top)};
+  return launched(name, i4::launch_token_logprobs(a, dtype, static_cast<cudaStream_t>(stream)));
 }
 
 int int4gemv_device_status(int* status) {

@@ -15,6 +15,7 @@ constexpr int kWarp = 32;
 constexpr int kStatusFullBarrierTimeout = 1;
 constexpr int kStatusEmptyBarrierTimeout = 2;
 constexpr int kStatusPeerTimeout = 3;  // a peer rank's flag did not arrive within the limit
+constexpr int kStatusBadPage = 4;  // a length or a block table entry outside of the cache
 
 // About one second at B200 clocks. A correct pipeline never waits more than microseconds.
 constexpr long long kWaitLimitCycles = 2000000000LL;

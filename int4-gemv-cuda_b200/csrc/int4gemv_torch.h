@@ -103,4 +103,37 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> repack_gptq(const at::Tensor& qwe
                                                           const at::Tensor& scales,
                                                           int64_t group_size, int64_t zero_offset);
 
+// ---- Decode-step operators around the GEMV (no counterpart in the reference) -------------------
+
+// (y, h): h = x + residual (x itself without one), y = h / rms(h) * weight, in x's type.
+std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const at::Tensor& weight,
+                                                double eps,
+                                                const c10::optional<at::Tensor>& residual);
+// (y, scales, h): y as e4m3 with one fp32 scale a row.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant(
+    const at::Tensor& x, const at::Tensor& weight, double eps,
+    const c10::optional<at::Tensor>& residual);
+
+// Attention of one new token a sequence, q [batch, q_heads, head_dim], over paged caches
+// [num_blocks, block_size, kv_heads, head_dim]. k, v [batch, kv_heads, head_dim]: the new tokens'
+// keys and values, written to the caches. weights [num_blocks, kv_heads, block_size] fp32: the
+// positions' attention weights are added to it.
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& block_table, const at::Tensor& seq_lens, double scale,
+                           const c10::optional<at::Tensor>& k, const c10::optional<at::Tensor>& v,
+                           const c10::optional<at::Tensor>& weights);
+
+// (kept, new_lens): the `recent` last positions and those of largest weight, `budget` in all,
+// copied to the pages of new_table.
+std::tuple<at::Tensor, at::Tensor> paged_evict(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                               const at::Tensor& weights,
+                                               const at::Tensor& block_table,
+                                               const at::Tensor& seq_lens, const at::Tensor& new_table,
+                                               int64_t budget, int64_t recent);
+
+// (logprobs, entropy, top_logprobs, top_ids) of the rows of logits.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const at::Tensor& logits,
+                                                                          const at::Tensor& tokens,
+                                                                          int64_t top);
+
 }  // namespace int4gemv

@@ -181,6 +181,76 @@ cudaError_t launch_repack(bool awq, uint32_t* qweight, half* scales, half* zeros
                           const half* ck_scales, int64_t n, int64_t k, int64_t group,
                           int zero_offset, cudaStream_t stream);
 
+// ---- Decode-step operators around the GEMV -------------------------------------------------------
+
+// Root-mean-square norm with the residual's addition (add_rms_norm.cu). x, residual, weight, h and
+// y are of one element type (WeightType); with scales, y is e4m3.
+struct NormArgs {
+  const void* x;         // [rows, hidden]
+  const void* residual;  // [rows, hidden] or null
+  const void* weight;    // [hidden]
+  void* h;               // [rows, hidden] or null; may be x or residual
+  void* y;               // [rows, hidden]
+  float* scales;         // [rows]: e4m3 output; or null
+  int rows, hidden;
+  float eps;
+  bool aligned;  // x, residual, weight, h and y start on a chunk boundary (16 bytes of x's type)
+};
+cudaError_t launch_add_rms_norm(const NormArgs& a, int dtype, cudaStream_t stream);
+
+// A paged cache of keys and values (paged_attention.cu, paged_evict.cu). Strides in elements; the
+// elements of one head are contiguous.
+struct PagedCache {
+  void* k;
+  void* v;
+  int64_t k_block, k_token, k_head;
+  int64_t v_block, v_token, v_head;
+  float* weights;  // [num_blocks, hkv, block_size] or null
+  int num_blocks, block_size, hkv, dim;
+};
+
+struct PagedAttentionArgs {
+  PagedCache cache;
+  void* out;         // [batch, hq, dim]
+  const void* q;     // [batch, hq, dim]
+  const int* table;  // [batch, max_blocks]
+  const int* lens;   // [batch]
+  const void* k_new;  // [batch, hkv, dim] or null
+  const void* v_new;
+  int batch, hq, max_blocks;
+  float scale_log2;  // the scale of the scores times log2(e)
+  void* workspace;
+};
+// Bytes of workspace a call needs; 0 if its sizes are out of the kernel's range.
+int64_t paged_attention_workspace_bytes(const PagedAttentionArgs& a);
+cudaError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, cudaStream_t stream);
+
+// Eviction from a paged cache by accumulated attention weight (paged_evict.cu).
+struct PagedEvictArgs {
+  PagedCache cache;
+  const int* table;      // [batch, max_blocks]
+  const int* lens;       // [batch]
+  const int* new_table;  // [batch, new_blocks]
+  int* kept;             // [batch, hkv, budget]
+  int* new_lens;         // [batch]
+  int batch, max_blocks, new_blocks, budget, recent;
+};
+cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream);
+
+// Log probabilities of given tokens, entropy and top alternatives (token_logprobs.cu).
+constexpr int kMaxTop = 32;
+struct LogprobArgs {
+  const void* logits;  // [rows, vocab], rows row_stride elements apart
+  const int64_t* tokens;
+  float* logprobs;      // [rows]
+  float* entropy;       // [rows]
+  float* top_logprobs;  // [rows, top]
+  int64_t* top_ids;     // [rows, top]
+  int64_t row_stride;
+  int rows, vocab, top;
+};
+cudaError_t launch_token_logprobs(const LogprobArgs& a, int dtype, cudaStream_t stream);
+
 // SM count of the current device (cached per device).
 int sm_count();
 

@@ -1,0 +1,248 @@
+// Eviction from a paged cache by accumulated attention weight. Per sequence and KV head, of n
+// positions the last `recent` stay, and of the older ones the budget - recent with the largest
+// weights (of equal ones the first); keys, values and weights of what stays go to the pages of a
+// new block table, in their old order.
+//
+// Two kernels. The choice: one block a (sequence, head), the k-th largest weight by a radix select
+// over the bits of the weights as ordered integers (11 + 11 + 10 bits, a histogram in shared memory
+// each), then the chosen positions in order by counting within and across warps. It reads 4 bytes
+// a position. The copy: a warp a (position, head), 16 bytes a lane, bound by HBM. The new pages are
+// not the old ones, so every block of the copy is independent of the others and sequences may
+// share old pages (a common prefix).
+#include <mutex>
+
+#include "decode.cuh"
+#include "kernels.h"
+
+namespace i4 {
+namespace {
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWarps = kSelectThreads / kWarp;
+constexpr int kBins = 2048;
+constexpr int kHeldKeys = 48 * 1024;  // weights kept in shared memory; longer ones are read again
+
+__device__ __forceinline__ void bad_page(int* status) { atomicExch(status, kStatusBadPage); }
+
+// Length of sequence b as the table can hold it.
+__device__ __forceinline__ int clamped_length(int n, int most, int* status) {
+  if (n < 0 || n > most) {
+    bad_page(status);
+    return n < 0 ? 0 : most;
+  }
+  return n;
+}
+
+__global__ void __launch_bounds__(kSelectThreads)
+    evict_select_kernel(const PagedEvictArgs a, int held, int* status) {
+  extern __shared__ uint32_t keys[];  // [held]
+  __shared__ int bins[kBins];
+  __shared__ int warp_gt[kSelectWarps], warp_eq[kSelectWarps], found_bin, found_above;
+  wait_then_release();
+  const int hkv = a.cache.hkv, page = a.cache.block_size;
+  const int b = blockIdx.x / hkv, head = blockIdx.x % hkv;
+  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+  const int64_t most = static_cast<int64_t>(a.max_blocks) * page;
+  const int n = clamped_length(a.lens[b], most < INT32_MAX ? static_cast<int>(most) : INT32_MAX,
+                               status);
+  const int kept = min(n, a.budget);
+  int* out = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  if (head == 0 && tid == 0) a.new_lens[b] = kept;
+  for (int j = kept + tid; j < a.budget; j += kSelectThreads) out[j] = -1;
+  if (n <= a.budget) {
+    for (int j = tid; j < kept; j += kSelectThreads) out[j] = j;
+    return;
+  }
+  const int recent = min(a.recent, a.budget);
+  const int old = n - recent;       // positions to choose from
+  const int want = kept - recent;   // how many of them stay (< old)
+  for (int j = tid; j < recent; j += kSelectThreads) out[want + j] = old + j;
+  if (want == 0) return;
+
+  const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
+  auto read_key = [&](int j) -> uint32_t {
+    const int p = table[j / page];
+    if (static_cast<unsigned>(p) >= static_cast<unsigned>(a.cache.num_blocks)) {
+      bad_page(status);
+      return 0;
+    }
+    return order_key(a.cache.weights[(static_cast<int64_t>(p) * hkv + head) * page + j % page]);
+  };
+  for (int j = tid; j < min(old, held); j += kSelectThreads) keys[j] = read_key(j);
+  auto key = [&](int j) { return j < held ? keys[j] : read_key(j); };
+
+  // the want-th largest key, digit by digit
+  uint32_t prefix = 0, mask = 0;
+  int left = want;  // rank still to find among the keys that match the prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int width = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+    __syncthreads();
+    for (int j = tid; j < old; j += kSelectThreads) {
+      const uint32_t k = key(j);
+      if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1);
+    }
+    __syncthreads();
+    // thread t owns bins 2 t and 2 t + 1 counted from the top; the sum of all bins above them
+    const int hi = kBins - 1 - 2 * tid;
+    const int own = bins[hi] + bins[hi - 1];
+    int upto = own;
+#pragma unroll
+    for (int off = 1; off < kWarp; off *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += v;
+    }
+    if (lane == kWarp - 1) warp_gt[warp] = upto;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += warp_gt[w];
+    const int above = before + upto - own;  // keys in bins above this thread's
+    if (above < left && left <= above + own) {
+      const bool first = left <= above + bins[hi];
+      found_bin = first ? hi : hi - 1;
+      found_above = first ? above : above + bins[hi];
+    }
+    __syncthreads();
+    left -= found_above;
+    prefix |= static_cast<uint32_t>(found_bin) << shift;
+    mask |= ((1u << width) - 1) << shift;
+    __syncthreads();
+  }
+  const uint32_t least = prefix;  // keys above it stay, and the first `left` of those equal to it
+
+  // each warp owns a contiguous range, so ranks follow from counts of the warps before it
+  const int range = ((old + kSelectWarps - 1) / kSelectWarps + kWarp - 1) / kWarp * kWarp;
+  const int j0 = min(warp * range, old), j1 = min(j0 + range, old);
+  int gt = 0, eq = 0;
+  for (int j = j0; j < j1; j += kWarp) {
+    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
+    gt += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k > least));
+    eq += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k == least));
+  }
+  if (lane == 0) {
+    warp_gt[warp] = gt;
+    warp_eq[warp] = eq;
+  }
+  __syncthreads();
+  int at = 0, eq_at = 0;
+  for (int w = 0; w < warp; ++w) {
+    at += warp_gt[w];
+    eq_at += warp_eq[w];
+  }
+  const uint32_t below = (1u << lane) - 1;
+  for (int j = j0; j < j1; j += kWarp) {
+    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
+    const uint32_t gts = __ballot_sync(0xffffffffu, j + lane < j1 && k > least);
+    const uint32_t eqs = __ballot_sync(0xffffffffu, j + lane < j1 && k == least);
+    const int my_eq = eq_at + __popc(eqs & below);
+    const bool stays = (gts >> lane & 1) || ((eqs >> lane & 1) && my_eq < left);
+    if (stays) out[at + __popc(gts & below) + min(my_eq, left)] = j + lane;
+    at += __popc(gts);
+    eq_at += __popc(eqs);
+  }
+}
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyRows = 4;  // rows a warp has in flight
+
+__global__ void __launch_bounds__(kCopyThreads)
+    evict_copy_kernel(const PagedEvictArgs a, int* status) {
+  wait_then_release();
+  const PagedCache& c = a.cache;
+  const int b = blockIdx.y, lane = threadIdx.x % kWarp;
+  const int kept = a.new_lens[b];
+  const int64_t rows = static_cast<int64_t>(kept) * c.hkv;
+  const int64_t first =
+      (static_cast<int64_t>(blockIdx.x) * (kCopyThreads / kWarp) + threadIdx.x / kWarp) * kCopyRows;
+  const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
+  const int* new_table = a.new_table + static_cast<int64_t>(b) * a.new_blocks;
+  const int vectors = c.dim / 8;  // of one row of keys
+  // elements are moved as 16-bit words of either type
+  const uint16_t* k = static_cast<const uint16_t*>(c.k);
+  const uint16_t* v = static_cast<const uint16_t*>(c.v);
+
+  struct Slot {
+    int page, offset;
+  };
+  Slot from[kCopyRows], to[kCopyRows];
+  int head[kCopyRows];  // -1: no row
+#pragma unroll
+  for (int i = 0; i < kCopyRows; ++i) {
+    head[i] = -1;
+    const int64_t r = first + i;
+    if (r >= rows) continue;
+    const int j = static_cast<int>(r / c.hkv), h = static_cast<int>(r % c.hkv);
+    const int src = a.kept[(static_cast<int64_t>(b) * c.hkv + h) * a.budget + j];
+    from[i] = {table[src / c.block_size], src % c.block_size};
+    to[i] = {new_table[j / c.block_size], j % c.block_size};
+    if (static_cast<unsigned>(from[i].page) >= static_cast<unsigned>(c.num_blocks) ||
+        static_cast<unsigned>(to[i].page) >= static_cast<unsigned>(c.num_blocks)) {
+      bad_page(status);
+    } else {
+      head[i] = h;
+    }
+  }
+  auto place = [&](const Slot& s, int h, bool value) {
+    return value ? s.page * c.v_block + s.offset * c.v_token + h * c.v_head
+                 : s.page * c.k_block + s.offset * c.k_token + h * c.k_head;
+  };
+  for (int i0 = lane; i0 < 2 * vectors; i0 += kWarp) {
+    const bool value = i0 >= vectors;
+    const int x = (value ? i0 - vectors : i0) * 8;
+    uint4 held[kCopyRows];
+#pragma unroll
+    for (int i = 0; i < kCopyRows; ++i) {
+      if (head[i] >= 0) {
+        held[i] = *reinterpret_cast<const uint4*>((value ? v : k) + place(from[i], head[i], value) + x);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCopyRows; ++i) {
+      if (head[i] >= 0) {
+        uint16_t* dst = static_cast<uint16_t*>(value ? c.v : c.k);
+        *reinterpret_cast<uint4*>(dst + place(to[i], head[i], value) + x) = held[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyRows; ++i) {
+    if (lane == i && head[i] >= 0) {
+      auto weight = [&](const Slot& s) -> float& {
+        return c.weights[(static_cast<int64_t>(s.page) * c.hkv + head[i]) * c.block_size + s.offset];
+      };
+      weight(to[i]) = weight(from[i]);
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
+  int* status = device_status_word();
+  if (!status) return cudaErrorInitializationError;
+  const int64_t most = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
+  const int held = static_cast<int>(most < kHeldKeys ? most : kHeldKeys);
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  std::call_once(once[dev & 63], [&] {
+    err = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kHeldKeys * 4);
+  });
+  if (err != cudaSuccess) return err;
+  err = launch_serialised(evict_select_kernel, dim3(a.batch * a.cache.hkv), dim3(kSelectThreads),
+                          static_cast<size_t>(held) * 4, stream, 1, a, held, status);
+  if (err != cudaSuccess) return err;
+  const int64_t longest = a.budget < most ? a.budget : most;
+  const int64_t rows = longest * a.cache.hkv;
+  if (rows == 0) return cudaSuccess;
+  const int per = kCopyThreads / kWarp * kCopyRows;
+  return launch_serialised(evict_copy_kernel,
+                           dim3(static_cast<unsigned>((rows + per - 1) / per), a.batch),
+                           dim3(kCopyThreads), 0, stream, 1, a, status);
+}
+
+}  // namespace i4

@@ -45,6 +45,16 @@ _PROTOTYPES = {
     "int4gemv_repack_gptq": (ctypes.c_int, [_p] * 6 + [ctypes.c_int] + [_i64] * 3 + [_p]),
     "int4gemv_quantize": (ctypes.c_int, [_p] * 4 + [ctypes.c_int] + [_i64] * 3 + [_p]),
     "int4gemv_pack": (ctypes.c_int, [_p, _p, _i64, _i64, _p]),
+    "int4gemv_add_rms_norm": (ctypes.c_int, [_p] * 5 + [ctypes.c_float, ctypes.c_int] + [_i64] * 2
+                              + [_p]),
+    "int4gemv_add_rms_norm_quant": (ctypes.c_int, [_p] * 6 + [ctypes.c_float, ctypes.c_int]
+                                    + [_i64] * 2 + [_p]),
+    "int4gemv_paged_cache_struct_bytes": (ctypes.c_size_t, []),
+    "int4gemv_paged_attention": (ctypes.c_int, [_p] * 5 + [ctypes.c_float] + [_p] * 2
+                                 + [ctypes.c_int] + [_i64] * 3 + [_p, _i64, _p]),
+    "int4gemv_paged_attention_workspace_size": (ctypes.c_int64, [_p] + [_i64] * 3 + [ctypes.c_int]),
+    "int4gemv_paged_evict": (ctypes.c_int, [_p] * 6 + [_i64] * 5 + [_p]),
+    "int4gemv_token_logprobs": (ctypes.c_int, [_p] * 6 + [ctypes.c_int] + [_i64] * 4 + [_p]),
     "int4gemv_device_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "int4gemv_set_strict_weights": (ctypes.c_int, [ctypes.c_int]),
     "int4gemv_peers_struct_bytes": (ctypes.c_size_t, []),
@@ -69,6 +79,18 @@ class Peers(ctypes.Structure):
                 ("reserved", ctypes.c_int32), ("n_total", ctypes.c_int64),
                 ("col0", ctypes.c_int64), ("out_bytes", ctypes.c_int64),
                 ("out", _p * MAX_PEERS), ("counters", _p)]
+
+
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+STATUS_BAD_PAGE = 4
+
+
+class PagedCache(ctypes.Structure):
+    """int4gemv_paged_cache_t."""
+
+    _fields_ = [("k", _p), ("v", _p), ("weights", _p), ("num_blocks", _i64), ("block_size", _i64),
+                ("kv_heads", _i64), ("head_dim", _i64), ("k_strides", _i64 * 3),
+                ("v_strides", _i64 * 3), ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class CapiError(RuntimeError):

@@ -4,8 +4,9 @@ Drop-in for the reference's int4gemv.ops (int4gemv/ops.py:11-36 of Yu-TingLee/in
 the same names (sequential, naive, coalesced, vectorized, load_only), the same KERNELS and
 KERNEL_INFO tables, plus the B200 fast path `w4a16`, the fused epilogues `w4a16_silu_mul` and
 `w4a16_bias_residual`, the unrounded fp32 row sums `w4a16_f32` (K-split partial sums), and the
-bit-exact device `quantize` / `pack` / `unpack` / `dequantize`. As
-in the reference, INT4GEMV_BUILD_DIR may point at another build directory (its `python/`
+bit-exact device `quantize` / `pack` / `unpack` / `dequantize`, and the decode step's operators
+between the GEMVs: `add_rms_norm` / `add_rms_norm_quant`, `paged_attention`, `paged_evict` and
+`token_logprobs`. As in the reference, INT4GEMV_BUILD_DIR may point at another build directory (its `python/`
 subdirectory or the directory itself is searched).
 
 There is no fallback: if the compiled module is missing this import fails and says how to build.
@@ -75,6 +76,11 @@ quantize = int4gemv_ops.quantize
 pack = int4gemv_ops.pack
 repack_awq = int4gemv_ops.repack_awq
 repack_gptq = int4gemv_ops.repack_gptq
+add_rms_norm = int4gemv_ops.add_rms_norm
+add_rms_norm_quant = int4gemv_ops.add_rms_norm_quant
+paged_attention = int4gemv_ops.paged_attention
+paged_evict = int4gemv_ops.paged_evict
+token_logprobs = int4gemv_ops.token_logprobs
 check_inputs = int4gemv_ops.check_inputs
 
 # The GEMV kernels, slowest first. All share the 5-argument signature of csrc/w4a16.h.
