@@ -7,7 +7,7 @@
 //
 // Bound by HBM: the cache is read once, 4 hq / hkv operations an element.
 //
-// Work: an item is (sequence, KV head, block of 16 query heads), cut into tiles of 64 positions.
+// Work: an item is (sequence, KV head, block of 8 or 16 query heads), cut into tiles of positions.
 // All tiles in order are split evenly over the blocks of the grid whatever the lengths are, so a
 // block works through the end of one item, whole items, and the beginning of another; an item that
 // several blocks share is joined by a second kernel from partial sums in the workspace, in block
@@ -16,10 +16,12 @@
 // A warp takes 16 positions of a tile and needs no other warp until its segment of an item ends:
 // it has its own ring of K and V tiles in shared memory, filled by cp.async (a row's page is looked
 // up while older tiles are in flight), its own running maximum and sum, and its own fp32
-// accumulators. S = Q K^T and O = P V are warp MMAs with the 16 query heads as rows (a KV head
-// with fewer leaves rows unused: the tensor pipe has several times the needed rate). P is given to
-// the MMA as a sum of two 16-bit numbers, so its rounding does not show in the result. Positions
-// behind the end are zero-filled in shared memory and masked, so nothing there reaches a sum.
+// accumulators. The warp MMAs have the positions and the dimensions as rows and 8 query heads as
+// columns: S^T = K Q^T, O^T = V^T P^T, so a group of 8 heads or fewer fills half of what heads as
+// rows would take (P^T gets from the first product's layout to the second's by movmatrix). P is
+// given to the MMA as a sum of two 16-bit numbers, so its rounding does not show in the result.
+// Positions behind the end are zero-filled in shared memory and masked, so nothing there reaches
+// a sum.
 #include <algorithm>
 #include <mutex>
 
@@ -29,38 +31,61 @@
 namespace i4 {
 namespace {
 
-constexpr int kRows = 16;       // query heads of an item
-constexpr int kWarpTile = 16;   // positions a warp takes of a tile
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * kWarp;
-constexpr int kTile = kWarps * kWarpTile;
+constexpr int kWarpTile = 16;  // positions a warp takes of a tile
 
-// Shapes by the head dimension rounded up: ring stages (their bytes in flight an SM), blocks an SM.
-constexpr int stages_of(int dp) { return dp == 256 ? 2 : 3; }
-constexpr int ctas_of(int dp) { return dp == 64 ? 3 : dp == 128 ? 2 : 1; }
+// What depends on the head dimension rounded up to DP and the heads of an item, 8 NT.
+template <int DP, int NT>
+struct Shape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kWarps = DP == 256 ? 6 : 4;
+  static constexpr int kThreads = kWarps * kWarp;
+  static constexpr int kTile = kWarps * kWarpTile;
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? (NT == 1 ? 3 : 2) : 1;  // of an SM
+  static constexpr int kChunks = DP / 8;                // 16-byte chunks of a row
+  static constexpr int kPitch = DP * 2 + 16;            // of a row in shared memory: the eight rows
+                                                        // of an ldmatrix fall into different banks
+  static constexpr int kHalf = kWarpTile * kPitch;      // K or V of a warp's tile
+  static constexpr bool kHoldQ = DP * NT <= 256;        // in registers; else in shared memory
+};
 constexpr int round_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// Unsigned division by a number known on the host, for dividends below 2^31 (Granlund and
+// Montgomery, Division by invariant integers using multiplication, 1994).
+struct Divider {
+  uint32_t mul, shift, by;
+  Divider() = default;
+  explicit Divider(uint32_t d) : by(d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << shift) - d) * (1ull << 32) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return (__umulhi(mul, n) + n) >> shift;
+  }
+};
 
 struct Plan {
   PagedAttentionArgs a;
   int group;       // query heads of a KV head
-  int head_tiles;  // blocks of 16 query heads of a KV head
+  int rows;        // query heads of an item, at most (8 or 16)
+  int head_tiles;  // items of a KV head
   int items;       // items of a sequence: hkv * head_tiles
+  int tile;        // positions of a tile
   int blocks;      // blocks of the attention kernel
   int max_len;     // positions the table has room for
-  float* part_o;   // [2 blocks][16][dim]: the segments of items that a block shares
-  float2* part_ml;  // [2 blocks][16]: their maximum (log2) and sum
-  float* lse;      // [batch][hq]: log2 of the sum, for items of one block (weights only)
-  float* scores;   // [tiles][min(group, 16)][64]: log2 scores (weights only)
+  int score_rows;  // heads of an item rounded up to a pair
+  Divider page;
+  float* part_o;    // [2 blocks][rows][dim]: the segments of items that a block shares
+  float2* part_ml;  // [2 blocks][rows]: their maximum (log2) and sum
+  float* lse;       // [batch][hq]: log2 of the sum, for items of one block (weights only)
+  float* scores;    // [tiles][tile][score_rows]: log2 scores (weights only)
   int* first_tile;  // [batch + 1]: tiles before each sequence
   int* status;
 };
 
-__device__ __forceinline__ int length_of(const Plan& p, int b) {
-  const int n = p.a.lens[b];
-  if (n < 0) return 0;
-  return n > p.max_len ? p.max_len : n;
-}
-__device__ __forceinline__ int tiles_of(int n) { return (n + kTile - 1) / kTile; }
+__device__ __forceinline__ int clamped(const Plan& p, int n) { return min(max(n, 0), p.max_len); }
+__device__ __forceinline__ int length_of(const Plan& p, int b) { return clamped(p, p.a.lens[b]); }
 
 // The even split of `total` tiles: block c takes [start(c), start(c + 1)).
 struct Split {
@@ -75,7 +100,11 @@ struct Split {
 
 // ---- Warp-level pieces ---------------------------------------------------------------------------
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Zeros where `there` is false; src is not read then.
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(there ? 16 : 0)
                : "memory");
@@ -98,6 +127,12 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "r"(addr)
                : "memory");
 }
+// The transpose of an 8 x 8 matrix of 16-bit numbers, a row of four lanes each.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
 template <class T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -119,155 +154,155 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
 struct Walker {
   int b, item, tile, tiles, n;
 
+  template <int kTile>
   __device__ __forceinline__ void enter(const Plan& p) {  // to the next sequence with positions
     while (b < p.a.batch) {
       n = length_of(p, b);
       if (n > 0) break;
       ++b;
     }
-    tiles = tiles_of(n);
+    tiles = (n + kTile - 1) / kTile;
   }
+  template <int kTile>
   __device__ __forceinline__ void next(const Plan& p) {
     if (++tile < tiles) return;
     tile = 0;
     if (++item < p.items) return;
     item = 0;
     ++b;
-    enter(p);
+    enter<kTile>(p);
   }
 };
 
-// Element size is 2 for both types: T only picks the MMA and the conversions.
-template <class T, int DP>
-struct Warp {
-  static constexpr int kRowBytes = DP * 2;
-  static constexpr int kTileBytes = kWarpTile * kRowBytes;  // K or V of a warp tile
-  static constexpr int kStages = stages_of(DP);
-  static constexpr int kChunks = DP / 8;
-  // 16-byte chunks of a row are stored at their index XOR the row's, so that the eight rows of an
-  // ldmatrix fall into different banks.
-  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
-    return row * kRowBytes + ((chunk ^ (row & 7)) << 4);
-  }
-};
-
-template <int DP>
+template <int DP, int NT>
 struct Smem {
-  static constexpr int kRing = kWarps * stages_of(DP) * 2 * kWarpTile * DP * 2;
-  alignas(1024) unsigned char ring[kRing];
-  const void* rows[kWarps][kWarpTile][2];  // K and V row of each position of the tile being loaded
-  uint32_t mask[kWarps][stages_of(DP)];    // positions that count
-  float joined[kRows][DP];
-  float2 ml[kWarps][kRows];
-  int scan[kWarps];
-  int start[3];  // sequence of the block's first tile, tiles before it, tiles in all
+  using S = Shape<DP, NT>;
+  alignas(128) unsigned char ring[S::kWarps][S::kStages][2][S::kHalf];
+  alignas(16) unsigned char q[S::kHoldQ ? 16 : S::kRows * S::kPitch];
+  const void* rows[S::kWarps][kWarpTile][2];  // K and V row of each position of the tile being loaded
+  uint32_t mask[S::kWarps][S::kStages];       // positions that count
+  float joined[S::kRows][DP];
+  float2 ml[S::kWarps][S::kRows];
+  int scan[S::kWarps];
+  int start[2];  // sequence of the block's first tile, tiles before it
 };
 
-template <class T, int DP, bool kWeights>
-__global__ void __launch_bounds__(kThreads, ctas_of(DP)) paged_attention_kernel(const Plan p) {
-  using W = Warp<T, DP>;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  Smem<DP>& sh = *reinterpret_cast<Smem<DP>*>(smem_raw);
+template <class T, int DP, int NT, bool kWeights>
+__global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
+    paged_attention_kernel(const __grid_constant__ Plan p) {
+  using S = Shape<DP, NT>;
+  constexpr int kTile = S::kTile, kThreads = S::kThreads, kWarps = S::kWarps;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  Smem<DP, NT>& sh = *reinterpret_cast<Smem<DP, NT>*>(smem_raw);
   wait_then_release();
   const PagedAttentionArgs& a = p.a;
   const PagedCache& c = a.cache;
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
 
-  // tiles in all
-  int total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-    int t = b0 + tid < a.batch ? tiles_of(length_of(p, b0 + tid)) * p.items : 0;
+  // Tiles before each sequence: a scan over the batch, a thread a sequence, in rounds. `find` is
+  // called with each thread's sequence and the tiles before and in it; returns the tiles in all.
+  auto scan = [&](auto find) {
+    int before = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+      const int b = b0 + tid;
+      const int given = b < a.batch ? a.lens[b] : 0;
+      const int n = clamped(p, given);
+      const int own = (n + kTile - 1) / kTile * p.items;
+      if (given != n && blockIdx.x == 0) atomicExch(p.status, kStatusBadPage);
+      int t = own;
 #pragma unroll
-    for (int off = 1; off < kWarp; off *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, t, off);
-      if (lane >= off) t += v;
+      for (int off = 1; off < kWarp; off *= 2) {
+        const int v = __shfl_up_sync(0xffffffffu, t, off);
+        if (lane >= off) t += v;
+      }
+      if (lane == kWarp - 1) sh.scan[warp] = t;
+      __syncthreads();
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) t += sh.scan[w];
+        sum += sh.scan[w];
+      }
+      if (b < a.batch) find(b, before + t - own, own);
+      before += sum;
+      __syncthreads();  // sh.scan is written again
     }
-    if (lane == kWarp - 1) sh.scan[warp] = t;
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) t += sh.scan[w];
-    }
+    return before;
+  };
+  // a batch that fits one round keeps the scan's result in registers
+  int my_b = -1, my_before = 0, my_own = 0;
+  const int total = scan([&](int b, int before, int own) {
     if (blockIdx.x == 0) {
-      if (b0 + tid < a.batch) p.first_tile[b0 + tid + 1] = total + t;
-      if (b0 + tid == 0) p.first_tile[0] = 0;
+      if (b == 0) p.first_tile[0] = 0;
+      p.first_tile[b + 1] = before + own;
     }
-    for (int w = 0; w < kWarps; ++w) total += sh.scan[w];
-    __syncthreads();
-  }
-  if (blockIdx.x == 0) {
-    for (int b = tid; b < a.batch; b += kThreads) {
-      if (a.lens[b] != length_of(p, b)) atomicExch(p.status, kStatusBadPage);
-    }
-  }
+    my_b = b;
+    my_before = before;
+    my_own = own;
+  });
   const Split split(total, p.blocks);
   const int t0 = split.start(blockIdx.x), t1 = split.start(blockIdx.x + 1);
   if (t0 >= t1) return;
-
-  // the sequence of tile t0
-  for (int b0 = 0, before = 0; b0 < a.batch; b0 += kThreads) {
-    const int own = b0 + tid < a.batch ? tiles_of(length_of(p, b0 + tid)) * p.items : 0;
-    int t = own;
-#pragma unroll
-    for (int off = 1; off < kWarp; off *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, t, off);
-      if (lane >= off) t += v;
+  auto is_start = [&](int b, int before, int own) {
+    if (before <= t0 && t0 < before + own) {
+      sh.start[0] = b;
+      sh.start[1] = before;
     }
-    if (lane == kWarp - 1) sh.scan[warp] = t;
+  };
+  if (a.batch <= kThreads) {
+    if (my_b >= 0) is_start(my_b, my_before, my_own);
     __syncthreads();
-    int sum = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) t += sh.scan[w];
-      sum += sh.scan[w];
-    }
-    t += before;
-    if (t - own <= t0 && t0 < t) {
-      sh.start[0] = b0 + tid;
-      sh.start[1] = t - own;
-    }
-    before += sum;
-    __syncthreads();
+  } else {
+    scan(is_start);
   }
   Walker load;
   load.b = sh.start[0];
-  load.enter(p);
+  load.enter<kTile>(p);
   load.item = (t0 - sh.start[1]) / load.tiles;
   load.tile = (t0 - sh.start[1]) % load.tiles;
   Walker now = load;
 
   // ---- loading
-  const uint32_t ring = smem_addr(sh.ring) + warp * W::kStages * 2 * W::kTileBytes;
+  const uint32_t ring = smem_addr(sh.ring[warp]);
   int load_tile = t0, load_stage = 0;
+  // the page of this lane's position in the tile to load next, read a tile ahead
+  auto position = [&] { return load.tile * kTile + warp * kWarpTile + lane; };
+  auto read_page = [&] {
+    const int pos = position();
+    return lane < kWarpTile && load_tile < t1 && pos < load.n
+               ? a.table[static_cast<int64_t>(load.b) * a.max_blocks + p.page.quotient(pos)]
+               : -1;
+  };
+  int page = read_page();
   auto load_next = [&] {
     if (load_tile < t1) {
       const int kv = load.item / p.head_tiles;
-      const int last = load.n - 1;
       bool valid = false, append = false;
       if (lane < kWarpTile) {
-        const int pos = load.tile * kTile + warp * kWarpTile + lane;
+        const int pos = position();
         const void* k = c.k;
         const void* v = c.v;
         if (pos < load.n) {
-          append = a.k_new != nullptr && pos == last;
-          const int page = a.table[static_cast<int64_t>(load.b) * a.max_blocks + pos / c.block_size];
           if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-            const int off = pos % c.block_size;
+            const int off = pos - p.page.quotient(pos) * p.page.by;
             valid = true;
+            append = a.k_new != nullptr && pos == load.n - 1;
             k = static_cast<const T*>(c.k) + page * c.k_block + off * c.k_token + kv * c.k_head;
             v = static_cast<const T*>(c.v) + page * c.v_block + off * c.v_token + kv * c.v_head;
           } else {
             atomicExch(p.status, kStatusBadPage);
           }
         }
-        sh.rows[warp][lane][0] = k;
-        sh.rows[warp][lane][1] = v;
+        *reinterpret_cast<ulonglong2*>(sh.rows[warp][lane]) =
+            make_ulonglong2(reinterpret_cast<uint64_t>(k), reinterpret_cast<uint64_t>(v));
       }
       const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-      const uint32_t fresh = __ballot_sync(0xffffffffu, valid && append);
+      const uint32_t fresh = __ballot_sync(0xffffffffu, append);
       if (lane == 0) sh.mask[warp][load_stage] = mask;
       __syncwarp();
-      const int64_t new_row = (static_cast<int64_t>(load.b) * c.hkv + kv) * c.dim;
       if (fresh) {
         // the new token's row: to its slot (once for a KV head), and read from the call's tensors
+        const int64_t new_row = (static_cast<int64_t>(load.b) * c.hkv + kv) * c.dim;
         const int row = __ffs(fresh) - 1;
         if (load.item % p.head_tiles == 0) {
           uint4* k = static_cast<uint4*>(const_cast<void*>(sh.rows[warp][row][0]));
@@ -284,158 +319,208 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) paged_attention_kernel(
         }
         __syncwarp();
       }
-      const uint32_t dst = ring + load_stage * 2 * W::kTileBytes;
+      load.next<kTile>(p);
+      ++load_tile;
+      page = read_page();
+      // a lane copies the same chunk of every kStep-th row
+      constexpr int kStep = kWarp / S::kChunks;
+      const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
+      const uint32_t dst = ring + load_stage * 2 * S::kHalf + row0 * S::kPitch + chunk * 16;
+      if (mask == 0xFFFFu && c.dim == DP) {
 #pragma unroll
-      for (int i = 0; i < kWarpTile * W::kChunks / kWarp; ++i) {
-        const int idx = i * kWarp + lane, row = idx / W::kChunks, chunk = idx % W::kChunks;
-        const bool there = (mask >> row & 1) && chunk * 8 < c.dim;
-        const T* k = static_cast<const T*>(sh.rows[warp][row][0]);
-        const T* v = static_cast<const T*>(sh.rows[warp][row][1]);
-        cp_async_16(dst + W::at(row, chunk), there ? k + chunk * 8 : k, there);
-        cp_async_16(dst + W::kTileBytes + W::at(row, chunk), there ? v + chunk * 8 : v, there);
+        for (int i = 0; i < kWarpTile / kStep; ++i) {
+          const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(sh.rows[warp][row0 + i * kStep]);
+          const uint32_t to = dst + i * kStep * S::kPitch;
+          cp_async_16(to, reinterpret_cast<const char*>(kv_row.x) + chunk * 16);
+          cp_async_16(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + chunk * 16);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = 0; i < kWarpTile / kStep; ++i) {
+          const int row = row0 + i * kStep;
+          const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(sh.rows[warp][row]);
+          const bool there = (mask >> row & 1) && chunk * 8 < c.dim;
+          const int at = there ? chunk * 16 : 0;
+          const uint32_t to = dst + i * kStep * S::kPitch;
+          cp_async_16_or_zero(to, reinterpret_cast<const char*>(kv_row.x) + at, there);
+          cp_async_16_or_zero(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + at, there);
+        }
       }
       __syncwarp();  // sh.rows is rewritten by the next load
-      load.next(p);
-      ++load_tile;
     }
     cp_async_commit();
-    load_stage = load_stage + 1 == W::kStages ? 0 : load_stage + 1;
+    load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
   };
 #pragma unroll
-  for (int s = 0; s < W::kStages - 1; ++s) load_next();
+  for (int s = 0; s < S::kStages - 1; ++s) load_next();
 
   // ---- computing
   const int g = lane / 4, t2 = lane % 4 * 2;
-  constexpr bool kHoldQ = DP <= 128;
-  uint32_t qf[kHoldQ ? DP / 16 : 1][4];
-  float o[DP / 8][4];
-  float m[2], l[2];
-  auto q_frag = [&](int k16, uint32_t (&f)[4]) {
-    const int kv = now.item / p.head_tiles;
-    const int h0 = now.item % p.head_tiles * kRows;
+  uint32_t qf[S::kHoldQ ? DP / 16 : 1][NT][2];
+  float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
+  float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the maximum of all lanes, this lane's sum
+  auto begin = [&] {
+    const int kv = now.item / p.head_tiles, h0 = now.item % p.head_tiles * S::kRows;
     const T* q = static_cast<const T*>(a.q) +
                  (static_cast<int64_t>(now.b) * a.hq + kv * p.group + h0) * c.dim;
+    if constexpr (S::kHoldQ) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = g + (i & 1) * 8, col = k16 * 16 + t2 + (i >> 1) * 8;
-      f[i] = h0 + row < p.group && col < c.dim
-                 ? *reinterpret_cast<const uint32_t*>(q + static_cast<int64_t>(row) * c.dim + col)
-                 : 0u;
-    }
-  };
-  auto begin = [&] {
-    if constexpr (kHoldQ) {
+      for (int k = 0; k < DP / 16; ++k) {
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) q_frag(k, qf[k]);
-    }
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    }
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.0f;
-  };
-  begin();
-  int stage = 0, segment = t0;  // first tile of the current segment
-  for (int t = t0; t < t1; ++t) {
-    cp_async_wait<W::kStages - 2>();
-    __syncwarp();
-    load_next();
-    const uint32_t ks = ring + stage * 2 * W::kTileBytes, vs = ks + W::kTileBytes;
-    const uint32_t mask = sh.mask[warp][stage];
-
-    // S: rows g and g + 8, positions t2, t2 + 1 of both halves of the 16
-    float s[2][4] = {};
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      if (k * 16 < c.dim) {
-        uint32_t b[4];
-        // matrices: positions 0-7 / k 0-7, positions 0-7 / k 8-15, positions 8-15 / ...
-        const int row = (lane & 7) + (lane >> 4) * 8, chunk = 2 * k + (lane >> 3 & 1);
-        ldmatrix_x4(b, ks + W::at(row, chunk));
-        uint32_t f[4];
-        if constexpr (kHoldQ) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] = qf[k][i];
-        } else {
-          q_frag(k, f);
-        }
-        mma<T>(s[0], f, b[0], b[1]);
-        mma<T>(s[1], f, b[2], b[3]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int pos = i * 8 + t2 + (j & 1);
-        s[i][j] = mask >> pos & 1 ? s[i][j] * a.scale_log2 : -INFINITY;
-      }
-    }
-    if constexpr (kWeights) {
-      const int rows = min(p.group, kRows);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (g + r * 8 < rows) {
-            float* to = p.scores + (static_cast<int64_t>(t) * rows + g + r * 8) * kTile +
-                        warp * kWarpTile + i * 8 + t2;
-            *reinterpret_cast<float2*>(to) = make_float2(s[i][2 * r], s[i][2 * r + 1]);
+          for (int j = 0; j < 2; ++j) {
+            const int row = i * 8 + g, col = k * 16 + j * 8 + t2;
+            qf[k][i][j] = h0 + row < p.group && col < c.dim
+                              ? *reinterpret_cast<const uint32_t*>(q + row * c.dim + col)
+                              : 0u;
           }
         }
       }
+    } else {
+      // every warp is past its use of the segment before (the join's barriers)
+      for (int i = tid; i < S::kRows * S::kChunks; i += kThreads) {
+        const int row = i / S::kChunks, chunk = i % S::kChunks;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (h0 + row < p.group && chunk * 8 < c.dim) {
+          v = *reinterpret_cast<const uint4*>(q + row * c.dim + chunk * 8);
+        }
+        *reinterpret_cast<uint4*>(sh.q + row * S::kPitch + chunk * 16) = v;
+      }
+      __syncthreads();
     }
-    float top[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      top[r] = fmaxf(top[r], m[r]);
+    for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - top[r]);
-        m[r] = top[r];
-        l[r] *= f;
+    for (int j = 0; j < NT; ++j) {
+      m[j][0] = m[j][1] = -INFINITY;
+      l[j][0] = l[j][1] = 0.0f;
+    }
+  };
+  begin();
+  // the lanes' rows and chunks in the ldmatrix of K (positions 0-7, 8-15 by k 0-7, then by 8-15)
+  // and of V (positions 0-7 by dims 0-7, by 8-15, then positions 8-15)
+  const uint32_t k_lane = ((lane & 7) + (lane >> 3 & 1) * 8) * S::kPitch + (lane >> 4) * 16;
+  const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16 + S::kHalf;
+
+  int stage = 0, segment = t0;  // first tile of the current segment
+  for (int t = t0; t < t1; ++t) {
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();
+    const uint32_t tile = ring + stage * 2 * S::kHalf;
+    const uint32_t mask = sh.mask[warp][stage];
+    load_next();
+
+    if (mask != 0 || kWeights) {
+      // S^T: positions g, g + 8 by heads t2, t2 + 1
+      float s[NT][4] = {};
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          o[i][2 * r] *= f;
-          o[i][2 * r + 1] *= f;
+      for (int k = 0; k < DP / 16; ++k) {
+        if (k * 16 < c.dim) {
+          uint32_t f[4];
+          ldmatrix_x4(f, tile + k_lane + k * 32);
+          if constexpr (S::kHoldQ) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) mma<T>(s[i], f, qf[k][i][0], qf[k][i][1]);
+          } else {
+            static_assert(S::kHoldQ || NT == 2, "an ldmatrix brings two blocks of heads");
+            uint32_t b[4];  // heads 0-7 by k 0-7, by 8-15, then heads 8-15
+            ldmatrix_x4(b, smem_addr(sh.q) + ((lane & 7) + (lane >> 4) * 8) * S::kPitch +
+                               (lane >> 3 & 1) * 16 + k * 32);
+            mma<T>(s[0], f, b[0], b[1]);
+            mma<T>(s[NT - 1], f, b[2], b[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] *= a.scale_log2;
+      }
+      if (mask != 0xFFFFu) {
+        const bool at[2] = {(mask >> g & 1) != 0, (mask >> (g + 8) & 1) != 0};
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = at[j / 2] ? s[i][j] : -INFINITY;
+        }
+      }
+      if constexpr (kWeights) {
+        float* to = p.scores + (static_cast<int64_t>(t) * kTile + warp * kWarpTile + g) * p.score_rows;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          if (i * 8 + t2 < p.score_rows) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              *reinterpret_cast<float2*>(to + r * 8 * p.score_rows + i * 8 + t2) =
+                  make_float2(s[i][2 * r], s[i][2 * r + 1]);
+            }
+          }
+        }
+      }
+      float top[NT][2];
+      bool rises = false;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float v = fmaxf(s[i][j], s[i][j + 2]);
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          top[i][j] = fmaxf(v, m[i][j]);
+          rises |= v > m[i][j];
+        }
+      }
+      if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float f = m[i][j] == -INFINITY ? 0.0f : exp2_fast(m[i][j] - top[i][j]);
+            m[i][j] = top[i][j];
+            l[i][j] *= f;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+              o[d][i][j] *= f;
+              o[d][i][j + 2] *= f;
+            }
+          }
+        }
+      }
+      uint32_t hi[NT][2], lo[NT][2];  // positions t2, t2 + 1 (and + 8) by head g
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const float ref0 = m[i][0] == -INFINITY ? 0.0f : m[i][0];
+        const float ref1 = m[i][1] == -INFINITY ? 0.0f : m[i][1];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float p0 = exp2_fast(s[i][2 * r] - ref0), p1 = exp2_fast(s[i][2 * r + 1] - ref1);
+          l[i][0] += p0;
+          l[i][1] += p1;
+          const uint32_t h = pack2<T>(p0, p1);
+          const float2 back = unpack2<T>(h);
+          hi[i][r] = transposed(h);
+          lo[i][r] = transposed(pack2<T>(p0 - back.x, p1 - back.y));
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        if (d * 16 < c.dim) {
+          uint32_t f[4];
+          ldmatrix_x4_trans(f, tile + v_lane + d * 32);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, hi[i][0], hi[i][1]);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, lo[i][0], lo[i][1]);
         }
       }
     }
-    const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float p0 = exp2_fast(s[i][2 * r] - ref[r]), p1 = exp2_fast(s[i][2 * r + 1] - ref[r]);
-        l[r] += p0 + p1;
-        hi[2 * i + r] = pack2<T>(p0, p1);
-        const float2 back = unpack2<T>(hi[2 * i + r]);
-        lo[2 * i + r] = pack2<T>(p0 - back.x, p1 - back.y);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 16; ++d) {
-      if (d * 16 < c.dim) {
-        uint32_t b[4];
-        // matrices: positions 0-7 / dims 0-7, positions 8-15 / dims 0-7, then dims 8-15
-        const int row = (lane & 7) + (lane >> 3 & 1) * 8, chunk = 2 * d + (lane >> 4);
-        ldmatrix_x4_trans(b, vs + W::at(row, chunk));
-        mma<T>(o[2 * d], hi, b[0], b[1]);
-        mma<T>(o[2 * d + 1], hi, b[2], b[3]);
-        mma<T>(o[2 * d], lo, b[0], b[1]);
-        mma<T>(o[2 * d + 1], lo, b[2], b[3]);
-      }
-    }
     __syncwarp();  // this stage is refilled by the next load_next
-    stage = stage + 1 == W::kStages ? 0 : stage + 1;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
     // ---- the end of a segment: join the warps
     const bool item_ends = now.tile + 1 == now.tiles;
@@ -444,59 +529,73 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) paged_attention_kernel(
       continue;
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (lane % 4 == 0) sh.ml[warp][g + r * 8] = make_float2(m[r], l[r]);
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 4);
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 8);
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 16);
+        if (g == 0) sh.ml[warp][i * 8 + t2 + j] = make_float2(m[i][j], l[i][j]);
+      }
     }
     __syncthreads();
-    float all_m[2], all_l[2], f[2];
+    float all_m[NT][2], all_l[NT][2], f[NT][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      all_m[r] = -INFINITY;
-      all_l[r] = 0.0f;
-      for (int w = 0; w < kWarps; ++w) all_m[r] = fmaxf(all_m[r], sh.ml[w][g + r * 8].x);
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 v = sh.ml[w][g + r * 8];
-        all_l[r] += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - all_m[r]);
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.ml[w][i * 8 + t2 + j].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 v = sh.ml[w][i * 8 + t2 + j];
+          sum += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - top);
+        }
+        all_m[i][j] = top;
+        all_l[i][j] = sum;
+        f[i][j] = m[i][j] == -INFINITY ? 1.0f : exp2_fast(m[i][j] - top);
       }
-      f[r] = m[r] == -INFINITY ? 1.0f : exp2_fast(m[r] - all_m[r]);
     }
     for (int w = 0; w < kWarps; ++w) {
       if (w == warp) {
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
+        for (int d = 0; d < DP / 16; ++d) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float2* to = reinterpret_cast<float2*>(&sh.joined[g + r * 8][i * 8 + t2]);
-            float2 v = make_float2(o[i][2 * r] * f[r], o[i][2 * r + 1] * f[r]);
-            if (w > 0) {
-              const float2 was = *to;
-              v.x += was.x;
-              v.y += was.y;
+          for (int i = 0; i < NT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float* to = &sh.joined[i * 8 + t2 + (j & 1)][d * 16 + g + j / 2 * 8];
+              const float v = o[d][i][j] * f[i][j & 1];
+              *to = w == 0 ? v : *to + v;
             }
-            *to = v;
           }
         }
       }
       __syncthreads();
     }
-    const int kv = now.item / p.head_tiles, h0 = now.item % p.head_tiles * kRows;
-    const int rows = min(p.group - h0, kRows);
-    const int head = kv * p.group + h0;
-    const bool whole = item_ends && t - segment + 1 == now.tiles;
-    if (lane % 4 == 0 && warp == 0) {  // rows g and g + 8 of this warp are the block's
+    if (warp == 0 && g == 0) {  // read by all warps above, before the loop's barriers
 #pragma unroll
-      for (int r = 0; r < 2; ++r) sh.ml[0][g + r * 8] = make_float2(all_m[r], all_l[r]);
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sh.ml[0][i * 8 + t2 + j] = make_float2(all_m[i][j], all_l[i][j]);
+        }
+      }
     }
     __syncthreads();
+    const int kv = now.item / p.head_tiles, h0 = now.item % p.head_tiles * S::kRows;
+    const int rows = min(p.group - h0, S::kRows);
+    const int head = kv * p.group + h0;
+    const bool whole = item_ends && t - segment + 1 == now.tiles;
     if (whole) {
       T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(now.b) * a.hq + head) * c.dim;
-      for (int i = tid; i < rows * (c.dim / 2); i += kThreads) {
-        const int row = i / (c.dim / 2), d = i % (c.dim / 2) * 2;
-        const float inv = 1.0f / sh.ml[0][row].y;
-        *reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(row) * c.dim + d) =
-            pack2<T>(sh.joined[row][d] * inv, sh.joined[row][d + 1] * inv);
+      const int pairs = c.dim / 2;
+      for (int i = tid; i < rows * pairs; i += kThreads) {
+        const int row = i / pairs, d = i % pairs * 2;
+        const float l_row = sh.ml[0][row].y;
+        *reinterpret_cast<uint32_t*>(out + row * c.dim + d) =
+            pack2<T>(sh.joined[row][d] / l_row, sh.joined[row][d + 1] / l_row);
       }
       if (kWeights && tid < rows) {
         p.lse[static_cast<int64_t>(now.b) * a.hq + head + tid] =
@@ -504,142 +603,194 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) paged_attention_kernel(
       }
     } else {
       const int slot = 2 * blockIdx.x + (segment == t0 ? 0 : 1);
-      float* to = p.part_o + static_cast<int64_t>(slot) * kRows * c.dim;
+      float* to = p.part_o + static_cast<int64_t>(slot) * S::kRows * c.dim;
       for (int i = tid; i < rows * c.dim; i += kThreads) to[i] = sh.joined[i / c.dim][i % c.dim];
-      if (tid < rows) p.part_ml[slot * kRows + tid] = sh.ml[0][tid];
+      if (tid < rows) p.part_ml[slot * S::kRows + tid] = sh.ml[0][tid];
     }
     __syncthreads();  // joined and ml are written again by the next segment
     if (t + 1 < t1) {
-      now.next(p);
+      now.next<kTile>(p);
       segment = t + 1;
       begin();
     }
   }
 }
 
-// Joins the items that several blocks share, zeroes the output of empty sequences, and (blocks
-// behind those of the items) adds the weights of the tiles.
+// ---- Joining -------------------------------------------------------------------------------------
+//
+// A block a (sequence, query head) joins what several blocks of the attention kernel hold of it:
+// the warps take the parts in turn, a lane four dimensions at a time, then the warps' sums are
+// added. It also zeroes the output of empty sequences. Blocks behind those add the weights: an even
+// share of the tiles each, a thread a position.
 constexpr int kJoinThreads = 128;
+constexpr int kJoinWarps = kJoinThreads / kWarp;
+constexpr int kMaxDim = 256;
 
-template <class T, bool kWeights>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Plan p) {
-  extern __shared__ float factor[];  // [16][blocks of an item]
-  __shared__ float row_lse[kRows];
-  wait_then_release();
+// Reads of the attention kernel's workspace
+struct Parts {
+  const Plan& p;
+  Split split;
+  int begin, o0, count;  // an item's first tile, its first block and the number of its blocks
+  __device__ __forceinline__ Parts(const Plan& plan, int total, int first, int tiles)
+      : p(plan), split(total, plan.blocks), begin(first), o0(split.owner(first)),
+        count(split.owner(first + tiles - 1) - o0 + 1) {}
+  __device__ __forceinline__ int64_t slot(int i) const {
+    return 2 * (o0 + i) + (split.start(o0 + i) >= begin ? 0 : 1);
+  }
+  // Maximum and sum of a row over all parts, by a whole warp.
+  __device__ __forceinline__ float2 row(int r, int lane) const {
+    float m = -INFINITY;
+    for (int i = lane; i < count; i += kWarp) m = fmaxf(m, p.part_ml[slot(i) * p.rows + r].x);
+#pragma unroll
+    for (int off = kWarp / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    float l = 0.0f;
+    for (int i = lane; i < count; i += kWarp) {
+      const float2 v = p.part_ml[slot(i) * p.rows + r];
+      l = fmaf(v.y, factor(v.x, m), l);
+    }
+    return make_float2(m, warp_sum(l));
+  }
+  // Of a part whose scores are all -inf nothing is scaled (its sums are 0, or NaN).
+  static __device__ __forceinline__ float factor(float m, float top) {
+    return m == -INFINITY ? 1.0f : exp2_fast(m - top);
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void join_head(const Plan& p, int index) {
+  __shared__ alignas(16) float sums[kJoinWarps][kMaxDim];
+  const PagedAttentionArgs& a = p.a;
+  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, dim = a.cache.dim;
+  const int b = index / a.hq, head = index % a.hq;
+  const int kv = head / p.group, h = head % p.group;
+  const int item = kv * p.head_tiles + h / p.rows, row = h % p.rows;
+  const int first = p.first_tile[b], tiles = (p.first_tile[b + 1] - first) / p.items;
+  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(index) * dim;
+  if (tiles == 0) {
+    for (int i = tid; i < dim; i += kJoinThreads) out[i] = from_f32<T>(0.0f);
+    return;
+  }
+  const Parts parts(p, p.first_tile[a.batch], first + item * tiles, tiles);
+  if (parts.count == 1) return;
+  const float2 ml = parts.row(row, lane);
+  float4 v[2] = {};
+#pragma unroll 4
+  for (int i = warp; i < parts.count; i += kJoinWarps) {
+    const int64_t at = parts.slot(i) * p.rows + row;
+    const float f = Parts::factor(p.part_ml[at].x, ml.x);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int d = (j * kWarp + lane) * 4;
+      if (d < dim) {
+        const float4 o = *reinterpret_cast<const float4*>(p.part_o + at * dim + d);
+        v[j].x = fmaf(o.x, f, v[j].x);
+        v[j].y = fmaf(o.y, f, v[j].y);
+        v[j].z = fmaf(o.z, f, v[j].z);
+        v[j].w = fmaf(o.w, f, v[j].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int d = (j * kWarp + lane) * 4;
+    if (d < dim) *reinterpret_cast<float4*>(&sums[warp][d]) = v[j];
+  }
+  __syncthreads();
+  for (int d = tid; d < dim; d += kJoinThreads) {
+    float sum = sums[0][d];
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) sum += sums[w][d];
+    out[d] = from_f32<T>(sum / ml.y);
+  }
+}
+
+__device__ __forceinline__ void add_weights(const Plan& p, int block, int blocks) {
+  __shared__ float row_lse[16];
+  __shared__ int start;
   const PagedAttentionArgs& a = p.a;
   const PagedCache& c = a.cache;
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+  // tiles of (sequence, KV head), the items of a KV head together
   const int total = p.first_tile[a.batch];
-  const Split split(total, p.blocks);
-
-  // the part of item (first tile `begin`) that block `o` holds
-  auto slot_of = [&](int o, int begin) { return 2 * o + (split.start(o) >= begin ? 0 : 1); };
-  // log2 of the item's sum for its rows, to row_lse, from blocks o0..o1; with kFactors also each
-  // part's share of the result
-  auto sums = [&](int begin, int o0, int o1, int rows, bool factors) {
-    const int parts = o1 - o0 + 1;
-    for (int row = warp; row < rows; row += kJoinThreads / kWarp) {
-      float m = -INFINITY;
-      for (int i = lane; i < parts; i += kWarp) {
-        m = fmaxf(m, p.part_ml[slot_of(o0 + i, begin) * kRows + row].x);
-      }
-#pragma unroll
-      for (int off = kWarp / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-      float l = 0.0f;
-      for (int i = lane; i < parts; i += kWarp) {
-        const float2 v = p.part_ml[slot_of(o0 + i, begin) * kRows + row];
-        const float f = v.x == -INFINITY ? 1.0f : exp2_fast(v.x - m);
-        if (factors) factor[row * parts + i] = f;
-        l = fmaf(v.y, f, l);
-      }
-      l = warp_sum(l);
-      if (lane == 0) row_lse[row] = factors ? l : m + log2f(l);
-    }
-    __syncthreads();
-  };
-
-  const int all_items = a.batch * p.items;
-  if (blockIdx.x < all_items) {
-    const int b = blockIdx.x / p.items, item = blockIdx.x % p.items;
-    const int kv = item / p.head_tiles, h0 = item % p.head_tiles * kRows;
-    const int rows = min(p.group - h0, kRows);
-    const int tiles = (p.first_tile[b + 1] - p.first_tile[b]) / p.items;
-    T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.hq + kv * p.group + h0) * c.dim;
-    if (tiles == 0) {
-      for (int i = tid; i < rows * c.dim; i += kJoinThreads) out[i] = from_f32<T>(0.0f);
-      return;
-    }
-    const int begin = p.first_tile[b] + item * tiles;
-    const int o0 = split.owner(begin), o1 = split.owner(begin + tiles - 1);
-    if (o0 == o1) return;
-    sums(begin, o0, o1, rows, true);
-    const int parts = o1 - o0 + 1;
-    for (int i = tid; i < rows * c.dim; i += kJoinThreads) {
-      const int row = i / c.dim;
-      float v = 0.0f;
-      for (int j = 0; j < parts; ++j) {
-        v = fmaf(p.part_o[static_cast<int64_t>(slot_of(o0 + j, begin)) * kRows * c.dim + i],
-                 factor[row * parts + j], v);
-      }
-      out[i] = from_f32<T>(v / row_lse[row]);
-    }
-    return;
+  const Split mine(total / p.head_tiles, blocks);
+  int t = mine.start(block);
+  const int t1 = mine.start(block + 1);
+  if (t >= t1) return;
+  for (int b = tid; b < a.batch; b += kJoinThreads) {
+    if (p.first_tile[b] / p.head_tiles <= t && t < p.first_tile[b + 1] / p.head_tiles) start = b;
   }
-
-  if constexpr (kWeights) {
-    // tiles of (sequence, KV head), the head tiles of a KV head together
-    const int kv_total = total / p.head_tiles;
-    const int blocks = gridDim.x - all_items, me = blockIdx.x - all_items;
-    const Split mine(kv_total, blocks);
-    int t = mine.start(me);
-    const int t1 = mine.start(me + 1);
-    if (t >= t1) return;
-    int b = 0;  // the sequence of tile t: the last whose tiles start at or before it
-    for (int step = 1 << 30; step > 0; step >>= 1) {
-      if (b + step < a.batch && p.first_tile[b + step] / p.head_tiles <= t) b += step;
-    }
-    while (t < t1) {
-      while (p.first_tile[b + 1] / p.head_tiles <= t) ++b;
-      const int n = length_of(p, b), tiles = tiles_of(n);
-      const int first = p.first_tile[b] / p.head_tiles;
-      const int kv = (t - first) / tiles, tile0 = (t - first) % tiles;
-      const int count = min(tiles - tile0, t1 - t);
-      for (int ht = 0; ht < p.head_tiles; ++ht) {
-        const int begin = p.first_tile[b] + (kv * p.head_tiles + ht) * tiles;
-        const int o0 = split.owner(begin), o1 = split.owner(begin + tiles - 1);
-        const int rows = min(p.group - ht * kRows, kRows);
-        if (o0 == o1) {
-          if (tid < rows) {
-            row_lse[tid] = p.lse[static_cast<int64_t>(b) * a.hq + kv * p.group + ht * kRows + tid];
-          }
-          __syncthreads();
-        } else {
-          sums(begin, o0, o1, rows, false);
+  __syncthreads();
+  int b = start;
+  while (t < t1) {
+    while (p.first_tile[b + 1] / p.head_tiles <= t) ++b;
+    const int n = length_of(p, b), tiles = (n + p.tile - 1) / p.tile;
+    const int first = p.first_tile[b] / p.head_tiles;
+    const int kv = (t - first) / tiles, tile0 = (t - first) % tiles;
+    const int count = min(tiles - tile0, t1 - t);
+    for (int ht = 0; ht < p.head_tiles; ++ht) {
+      const int begin = p.first_tile[b] + (kv * p.head_tiles + ht) * tiles;
+      const int rows = min(p.group - ht * p.rows, p.rows);
+      const Parts parts(p, total, begin, tiles);
+      if (parts.count == 1) {
+        if (tid < rows) {
+          row_lse[tid] = p.lse[static_cast<int64_t>(b) * a.hq + kv * p.group + ht * p.rows + tid];
         }
-        const int stride = min(p.group, kRows);
-        for (int i = tid; i < count * kTile; i += kJoinThreads) {
-          const int tile = tile0 + i / kTile, pos = tile * kTile + i % kTile;
-          if (pos < n) {
-            const float* s = p.scores + static_cast<int64_t>(begin + tile) * stride * kTile + i % kTile;
-            float w = 0.0f;
-            for (int row = 0; row < rows; ++row) w += exp2_fast(s[row * kTile] - row_lse[row]);
-            const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + pos / c.block_size];
-            if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-              float* to = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
-                          pos % c.block_size;
-              // a new token's slot may hold what its page was used for before
-              *to = ht == 0 && a.k_new && pos == n - 1 ? w : *to + w;
-            }
-          }
+      } else {
+        for (int r = warp; r < rows; r += kJoinWarps) {
+          const float2 ml = parts.row(r, lane);
+          if (lane == 0) row_lse[r] = ml.x + log2f(ml.y);
         }
-        __syncthreads();  // row_lse is rewritten
       }
-      t += count;
+      __syncthreads();
+      for (int i = tid; i < count * p.tile; i += kJoinThreads) {
+        const int pos = tile0 * p.tile + i;
+        if (pos >= n) break;
+        const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + p.page.quotient(pos)];
+        const float2* s = reinterpret_cast<const float2*>(
+            p.scores + (static_cast<int64_t>(begin + tile0) * p.tile + i) * p.score_rows);
+        float w = 0.0f;
+#pragma unroll 4
+        for (int r = 0; r < rows; r += 2) {
+          const float2 v = s[r / 2];
+          w += exp2_fast(v.x - row_lse[r]);
+          if (r + 1 < rows) w += exp2_fast(v.y - row_lse[r + 1]);
+        }
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
+          float* to = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
+                      (pos - p.page.quotient(pos) * p.page.by);
+          // a new token's slot may hold what its page was used for before
+          *to = ht == 0 && a.k_new && pos == n - 1 ? w : *to + w;
+        }
+      }
+      __syncthreads();  // row_lse is rewritten
     }
+    t += count;
+  }
+}
+
+template <class T, bool kWeights>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Plan p) {
+  wait_then_release();
+  const int heads = p.a.batch * p.a.hq;
+  if (static_cast<int>(blockIdx.x) < heads) {
+    join_head<T>(p, blockIdx.x);
+  } else if constexpr (kWeights) {
+    add_weights(p, blockIdx.x - heads, gridDim.x - heads);
   }
 }
 
 // ---- Host ----------------------------------------------------------------------------------------
+
+// Calls f with the Shape of a call as template arguments <DP, NT>.
+template <class F>
+auto with_shape(int dim, int group, F f) {
+  const bool wide = group > 8;
+  switch (round_dim(dim)) {
+    case 64: return wide ? f.template operator()<64, 2>() : f.template operator()<64, 1>();
+    case 128: return wide ? f.template operator()<128, 2>() : f.template operator()<128, 1>();
+    default: return wide ? f.template operator()<256, 2>() : f.template operator()<256, 1>();
+  }
+}
 
 int64_t aligned_up(int64_t n) { return (n + 255) / 256 * 256; }
 
@@ -647,14 +798,25 @@ int64_t aligned_up(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
   p->a = a;
   p->group = a.hq / a.cache.hkv;
-  p->head_tiles = (p->group + kRows - 1) / kRows;
+  int ctas = 1;
+  with_shape(a.cache.dim, p->group, [&]<int DP, int NT>() {
+    p->rows = Shape<DP, NT>::kRows;
+    p->tile = Shape<DP, NT>::kTile;
+    ctas = Shape<DP, NT>::kCtas;
+  });
+  p->head_tiles = (p->group + p->rows - 1) / p->rows;
   const int64_t items = static_cast<int64_t>(a.cache.hkv) * p->head_tiles;
   const int64_t len = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
-  const int64_t tiles = a.batch * items * ((len + kTile - 1) / kTile);
-  if (len > INT32_MAX - kTile || tiles > INT32_MAX / 2 || a.batch * items > INT32_MAX / 4) return 0;
+  const int64_t tiles = a.batch * items * ((len + p->tile - 1) / p->tile);
+  if (len > INT32_MAX - p->tile || tiles > INT32_MAX / 2 ||
+      static_cast<int64_t>(a.batch) * a.hq > INT32_MAX / 4) {
+    return 0;
+  }
   p->items = static_cast<int>(items);
   p->max_len = static_cast<int>(len);
-  const int64_t resident = static_cast<int64_t>(sm_count()) * ctas_of(round_dim(a.cache.dim));
+  p->score_rows = (std::min(p->group, p->rows) + 1) / 2 * 2;
+  p->page = Divider(static_cast<uint32_t>(a.cache.block_size));
+  const int64_t resident = static_cast<int64_t>(sm_count()) * ctas;
   p->blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, tiles)));
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -662,49 +824,34 @@ int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
     at += aligned_up(bytes);
     return static_cast<unsigned char*>(a.workspace) + here;
   };
-  p->part_o = reinterpret_cast<float*>(take(2LL * p->blocks * kRows * a.cache.dim * 4));
-  p->part_ml = reinterpret_cast<float2*>(take(2LL * p->blocks * kRows * 8));
+  p->part_o = reinterpret_cast<float*>(take(2LL * p->blocks * p->rows * a.cache.dim * 4));
+  p->part_ml = reinterpret_cast<float2*>(take(2LL * p->blocks * p->rows * 8));
   p->first_tile = reinterpret_cast<int*>(take((a.batch + 1LL) * 4));
   if (a.cache.weights) {
     p->lse = reinterpret_cast<float*>(take(static_cast<int64_t>(a.batch) * a.hq * 4));
-    p->scores = reinterpret_cast<float*>(
-        take(tiles * std::min(p->group, kRows) * kTile * 4));
+    p->scores = reinterpret_cast<float*>(take(tiles * p->tile * p->score_rows * 4));
   }
   return at;
 }
 
-template <class T, int DP, bool kWeights>
+template <class T, int DP, int NT, bool kWeights>
 cudaError_t launch(const Plan& p, cudaStream_t stream) {
   static std::once_flag once[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   std::call_once(once[dev & 63], [&] {
-    err = cudaFuncSetAttribute(paged_attention_kernel<T, DP, kWeights>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<DP>));
+    err = cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT, kWeights>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<DP, NT>));
   });
   if (err != cudaSuccess) return err;
-  err = launch_serialised(paged_attention_kernel<T, DP, kWeights>, dim3(p.blocks), dim3(kThreads),
-                          sizeof(Smem<DP>), stream, 1, p);
+  err = launch_serialised(paged_attention_kernel<T, DP, NT, kWeights>, dim3(p.blocks),
+                          dim3(Shape<DP, NT>::kThreads), sizeof(Smem<DP, NT>), stream, 1, p);
   if (err != cudaSuccess) return err;
-  const unsigned items = static_cast<unsigned>(p.a.batch) * p.items;
+  const int heads = p.a.batch * p.a.hq;
   return launch_serialised(paged_join_kernel<T, kWeights>,
-                           dim3(items + (kWeights ? p.blocks : 0)), dim3(kJoinThreads),
-                           static_cast<size_t>(p.blocks) * kRows * 4, stream, 1, p);
-}
-
-template <class T, bool kWeights>
-cudaError_t launch_dim(const Plan& p, cudaStream_t stream) {
-  switch (round_dim(p.a.cache.dim)) {
-    case 64: return launch<T, 64, kWeights>(p, stream);
-    case 128: return launch<T, 128, kWeights>(p, stream);
-    default: return launch<T, 256, kWeights>(p, stream);
-  }
-}
-
-template <class T>
-cudaError_t launch_type(const Plan& p, cudaStream_t stream) {
-  return p.a.cache.weights ? launch_dim<T, true>(p, stream) : launch_dim<T, false>(p, stream);
+                           dim3(heads + (kWeights ? 4 * sm_count() : 0)), dim3(kJoinThreads), 0,
+                           stream, 1, p);
 }
 
 }  // namespace
@@ -719,7 +866,14 @@ cudaError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, cudaS
   make_plan(a, &p);
   p.status = device_status_word();
   if (!p.status) return cudaErrorInitializationError;
-  return dtype == kWeightF16 ? launch_type<half>(p, stream) : launch_type<__nv_bfloat16>(p, stream);
+  return with_shape(a.cache.dim, p.group, [&]<int DP, int NT>() {
+    if (dtype == kWeightF16) {
+      return a.cache.weights ? launch<half, DP, NT, true>(p, stream)
+                             : launch<half, DP, NT, false>(p, stream);
+    }
+    return a.cache.weights ? launch<__nv_bfloat16, DP, NT, true>(p, stream)
+                           : launch<__nv_bfloat16, DP, NT, false>(p, stream);
+  });
 }
 
 }  // namespace i4
