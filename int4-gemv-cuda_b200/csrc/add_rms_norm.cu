@@ -5,11 +5,14 @@
 // its squares and the store. The 8-bit output needs max|y| = max|h w| / rms, so the same reduction
 // carries max|h w| beside the sum and the row still needs no second one.
 //
-// Layout: the row is cut into the 16-byte chunks of memory it lies in, so that a row of odd length
-// (whose start falls inside a chunk) still moves whole chunks; only its first and last chunk go by
-// elements.
+// Layout: rows of whole 16-byte chunks go to blocks that stay for many rows: a thread holds its
+// chunks of the weight throughout and fetches the next row while this one is summed and stored.
+// Other rows (odd lengths, unaligned tensors) are cut into the chunks of memory they lie in, so that
+// they still move whole chunks and only their first and last one by elements.
 //
 // Bound by HBM: x, residual, h and y move once each.
+#include <algorithm>
+
 #include "decode.cuh"
 #include "kernels.h"
 
@@ -17,6 +20,7 @@ namespace i4 {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
+constexpr int kRowThreads = 1024;  // threads an SM gets for rows of whole chunks
 constexpr float kScaleFloor = 1e-12f;  // a row of zeros still has a scale to divide by
 
 // Four / eight e4m3 values of y, saturating (a NaN stays one).
@@ -215,11 +219,112 @@ __global__ void __launch_bounds__(kRows > 1 ? kRows * kWarp : 1024)
   }
 }
 
+// Rows of whole chunks. kPer chunks a thread, blocks of as many threads as a row needs; rows are
+// taken in turn by the blocks of the grid.
+template <class T, bool Q8, bool kResidual, int kPer>
+__global__ void __launch_bounds__(1024) add_rms_norm_rows_kernel(const NormArgs a) {
+  __shared__ float2 scratch[2][kWarp];
+  wait_then_release();
+  constexpr int E = Chunk<T>::kElems;
+  const int chunks = a.hidden / E, tid = threadIdx.x;
+  const int warps = blockDim.x / kWarp;
+  const uint4* x = static_cast<const uint4*>(a.x);
+  const uint4* residual = static_cast<const uint4*>(a.residual);
+  const uint4* weight = static_cast<const uint4*>(a.weight);
+
+  uint4 w[kPer], nx[kPer], nr[kPer];
+  auto fetch = [&](int64_t row) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int c = tid + j * blockDim.x;
+      if (c < chunks) {
+        nx[j] = ld_stream_v4(x + row * chunks + c);
+        if (kResidual) nr[j] = ld_stream_v4(residual + row * chunks + c);
+      }
+    }
+  };
+  int64_t row = blockIdx.x;
+  fetch(row);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const int c = tid + j * blockDim.x;
+    w[j] = c < chunks ? weight[c] : make_uint4(0, 0, 0, 0);
+  }
+  for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+    Chunk<T> h[kPer];
+    float sum = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (tid + j * static_cast<int>(blockDim.x) >= chunks) continue;
+      h[j].set(nx[j]);
+      if (kResidual) {
+        Chunk<T> r;
+        r.set(nr[j]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) h[j].v[i] += r.v[i];
+      }
+      Chunk<T> wc;
+      if (Q8) wc.set(w[j]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        sum = fmaf(h[j].v[i], h[j].v[i], sum);
+        if (Q8) top = max_nan(top, fabsf(h[j].v[i] * wc.v[i]));
+      }
+    }
+    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    // two scratch rows in turn: a warp writes one again only after a barrier behind its reads
+    row_reduce(sum, top, warps, scratch[turn]);
+    float rstd = rsqrtf(sum / static_cast<float>(a.hidden) + a.eps);
+    if constexpr (Q8) {
+      float scale = rstd * top / kE4m3Max;
+      if (scale < kScaleFloor) scale = kScaleFloor;  // written so that a NaN stays one
+      if (tid == 0) a.scales[row] = scale;
+      rstd = rstd / scale;
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int c = tid + j * blockDim.x;
+      if (c >= chunks) continue;
+      if (kResidual) static_cast<uint4*>(a.h)[row * chunks + c] = h[j].get();
+      Chunk<T> y;
+      y.set(w[j]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) y.v[i] = h[j].v[i] * rstd * y.v[i];
+      if constexpr (!Q8) {
+        static_cast<uint4*>(a.y)[row * chunks + c] = y.get();
+      } else {
+        uint32_t* to = static_cast<uint32_t*>(a.y) + (row * chunks + c) * (E / 4);
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(y.v[0], y.v[1], y.v[2], y.v[3]),
+                                                     e4m3x4(y.v[4], y.v[5], y.v[6], y.v[7]));
+        } else {
+          *to = e4m3x4(y.v[0], y.v[1], y.v[2], y.v[3]);
+        }
+      }
+    }
+  }
+}
+
 template <class T, bool Q8>
 cudaError_t launch(const NormArgs& a, cudaStream_t stream) {
   constexpr int E = Chunk<T>::kElems;
-  const int most = (E - 1 + a.hidden + E - 1) / E;  // chunks of a row at any shift
   const auto up = [](int n, int to) { return (n + to - 1) / to * to; };
+  // without a residual h is x, and a caller that asks for it gets a copy from the general kernel
+  if (a.aligned && a.hidden % E == 0 && a.hidden / E <= 2048 && (a.residual || !a.h)) {
+    const int chunks = a.hidden / E;
+    const auto rows = [&](auto with, auto without, int per) {
+      const int threads = up((chunks + per - 1) / per, kWarp);
+      const int ctas = std::max(1, kRowThreads / threads) * sm_count();
+      return launch_serialised(a.residual ? with : without, dim3(std::min(a.rows, ctas)),
+                               dim3(threads), 0, stream, 1, a);
+    };
+    const bool few = a.rows <= sm_count();
+    if (chunks <= 256 || (few && chunks <= 1024)) {
+      return rows(add_rms_norm_rows_kernel<T, Q8, true, 1>, add_rms_norm_rows_kernel<T, Q8, false, 1>, 1);
+    }
+    return rows(add_rms_norm_rows_kernel<T, Q8, true, 2>, add_rms_norm_rows_kernel<T, Q8, false, 2>, 2);
+  }
+  const int most = (E - 1 + a.hidden + E - 1) / E;  // chunks of a row at any shift
   if (most <= kWarp * 4 && a.rows > 1) {
     constexpr int kRows = 4;
     return launch_serialised(add_rms_norm_kernel<T, Q8, 4, kRows>,

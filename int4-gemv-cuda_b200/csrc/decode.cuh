@@ -124,6 +124,21 @@ __device__ __forceinline__ float from_order_key(uint32_t k) {
   return __uint_as_float(k >> 31 ? k ^ 0x80000000u : ~k);
 }
 
+// Unsigned division by a number known on the host, for dividends below 2^31 (Granlund and
+// Montgomery, Division by invariant integers using multiplication, 1994).
+struct Divider {
+  uint32_t mul, shift, by;
+  Divider() = default;
+  explicit Divider(uint32_t d) : by(d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << shift) - d) * (1ull << 32) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return (__umulhi(mul, n) + n) >> shift;
+  }
+};
+
 // ---- Launch -------------------------------------------------------------------------------------
 
 // Launches `kernel` with programmatic stream serialization (see wait_then_release), its blocks

@@ -50,21 +50,6 @@ struct Shape {
 };
 constexpr int round_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-// Unsigned division by a number known on the host, for dividends below 2^31 (Granlund and
-// Montgomery, Division by invariant integers using multiplication, 1994).
-struct Divider {
-  uint32_t mul, shift, by;
-  Divider() = default;
-  explicit Divider(uint32_t d) : by(d) {
-    shift = 0;
-    while ((1ull << shift) < d) ++shift;
-    mul = static_cast<uint32_t>(((1ull << shift) - d) * (1ull << 32) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
-    return (__umulhi(mul, n) + n) >> shift;
-  }
-};
-
 struct Plan {
   PagedAttentionArgs a;
   int group;       // query heads of a KV head

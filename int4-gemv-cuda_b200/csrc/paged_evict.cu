@@ -20,6 +20,7 @@ namespace {
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / kWarp;
 constexpr int kBins = 2048;
+constexpr int kReads = 8;  // weights a thread has in flight
 constexpr int kHeldKeys = 48 * 1024;  // weights kept in shared memory; longer ones are read again
 
 __device__ __forceinline__ void bad_page(int* status) { atomicExch(status, kStatusBadPage); }
@@ -34,7 +35,7 @@ __device__ __forceinline__ int clamped_length(int n, int most, int* status) {
 }
 
 __global__ void __launch_bounds__(kSelectThreads)
-    evict_select_kernel(const PagedEvictArgs a, int held, int* status) {
+    evict_select_kernel(const PagedEvictArgs a, const Divider by_page, int held, int* status) {
   extern __shared__ uint32_t keys[];  // [held]
   __shared__ int bins[kBins];
   __shared__ int warp_gt[kSelectWarps], warp_eq[kSelectWarps], found_bin, found_above;
@@ -61,14 +62,26 @@ __global__ void __launch_bounds__(kSelectThreads)
 
   const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
   auto read_key = [&](int j) -> uint32_t {
-    const int p = table[j / page];
+    const int block = by_page.quotient(j), p = table[block];
     if (static_cast<unsigned>(p) >= static_cast<unsigned>(a.cache.num_blocks)) {
       bad_page(status);
       return 0;
     }
-    return order_key(a.cache.weights[(static_cast<int64_t>(p) * hkv + head) * page + j % page]);
+    return order_key(a.cache.weights[(static_cast<int64_t>(p) * hkv + head) * page + j - block * page]);
   };
-  for (int j = tid; j < min(old, held); j += kSelectThreads) keys[j] = read_key(j);
+  for (int j0 = tid; j0 < min(old, held); j0 += kReads * kSelectThreads) {
+    uint32_t k[kReads];  // kept apart from the stores, so that the reads do not wait for each other
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      const int j = j0 + i * kSelectThreads;
+      k[i] = j < min(old, held) ? read_key(j) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      const int j = j0 + i * kSelectThreads;
+      if (j < min(old, held)) keys[j] = k[i];
+    }
+  }
   auto key = [&](int j) { return j < held ? keys[j] : read_key(j); };
 
   // the want-th largest key, digit by digit
@@ -145,74 +158,69 @@ __global__ void __launch_bounds__(kSelectThreads)
 }
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyRows = 4;  // rows a warp has in flight
+constexpr int kCopyWarps = kCopyThreads / kWarp;
+constexpr int kCopyRows = 8;  // positions a warp has in flight
 
 __global__ void __launch_bounds__(kCopyThreads)
-    evict_copy_kernel(const PagedEvictArgs a, int* status) {
+    evict_copy_kernel(const PagedEvictArgs a, const Divider by_page, int* status) {
   wait_then_release();
   const PagedCache& c = a.cache;
-  const int b = blockIdx.y, lane = threadIdx.x % kWarp;
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  const int b = blockIdx.y;
   const int kept = a.new_lens[b];
-  const int64_t rows = static_cast<int64_t>(kept) * c.hkv;
-  const int64_t first =
-      (static_cast<int64_t>(blockIdx.x) * (kCopyThreads / kWarp) + threadIdx.x / kWarp) * kCopyRows;
+  const int j0 = blockIdx.x * kWarp;
+  if (j0 >= kept) return;
   const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
   const int* new_table = a.new_table + static_cast<int64_t>(b) * a.new_blocks;
-  const int vectors = c.dim / 8;  // of one row of keys
   // elements are moved as 16-bit words of either type
   const uint16_t* k = static_cast<const uint16_t*>(c.k);
   const uint16_t* v = static_cast<const uint16_t*>(c.v);
+  const int vectors = c.dim / 8;  // 16-byte pieces of a row of keys
+  const int count = min(kWarp, kept - j0);
 
-  struct Slot {
-    int page, offset;
-  };
-  Slot from[kCopyRows], to[kCopyRows];
-  int head[kCopyRows];  // -1: no row
-#pragma unroll
-  for (int i = 0; i < kCopyRows; ++i) {
-    head[i] = -1;
-    const int64_t r = first + i;
-    if (r >= rows) continue;
-    const int j = static_cast<int>(r / c.hkv), h = static_cast<int>(r % c.hkv);
-    const int src = a.kept[(static_cast<int64_t>(b) * c.hkv + h) * a.budget + j];
-    from[i] = {table[src / c.block_size], src % c.block_size};
-    to[i] = {new_table[j / c.block_size], j % c.block_size};
-    if (static_cast<unsigned>(from[i].page) >= static_cast<unsigned>(c.num_blocks) ||
-        static_cast<unsigned>(to[i].page) >= static_cast<unsigned>(c.num_blocks)) {
-      bad_page(status);
-    } else {
-      head[i] = h;
-    }
-  }
-  auto place = [&](const Slot& s, int h, bool value) {
-    return value ? s.page * c.v_block + s.offset * c.v_token + h * c.v_head
-                 : s.page * c.k_block + s.offset * c.k_token + h * c.k_head;
-  };
-  for (int i0 = lane; i0 < 2 * vectors; i0 += kWarp) {
-    const bool value = i0 >= vectors;
-    const int x = (value ? i0 - vectors : i0) * 8;
-    uint4 held[kCopyRows];
-#pragma unroll
-    for (int i = 0; i < kCopyRows; ++i) {
-      if (head[i] >= 0) {
-        held[i] = *reinterpret_cast<const uint4*>((value ? v : k) + place(from[i], head[i], value) + x);
+  for (int h = warp; h < c.hkv; h += kCopyWarps) {
+    // this lane's position: where it is and where it goes
+    int from_page = -1, from_off = 0, to_page = -1, to_off = 0;
+    if (lane < count) {
+      const int j = j0 + lane;
+      const int src = a.kept[(static_cast<int64_t>(b) * c.hkv + h) * a.budget + j];
+      const int sb = by_page.quotient(src), db = by_page.quotient(j);
+      from_page = table[sb];
+      to_page = new_table[db];
+      from_off = src - sb * c.block_size;
+      to_off = j - db * c.block_size;
+      if (static_cast<unsigned>(from_page) >= static_cast<unsigned>(c.num_blocks) ||
+          static_cast<unsigned>(to_page) >= static_cast<unsigned>(c.num_blocks)) {
+        bad_page(status);
+        from_page = -1;
+      } else {
+        c.weights[(static_cast<int64_t>(to_page) * c.hkv + h) * c.block_size + to_off] =
+            c.weights[(static_cast<int64_t>(from_page) * c.hkv + h) * c.block_size + from_off];
       }
     }
+    for (int i0 = lane; i0 < 2 * vectors + lane; i0 += kWarp) {  // all lanes take part in the shuffles
+      const bool inside = i0 < 2 * vectors, value = i0 >= vectors;
+      const int x = (value ? i0 - vectors : i0) * 8;
+      const uint16_t* src = (value ? v : k) + h * (value ? c.v_head : c.k_head) + x;
+      uint16_t* dst = static_cast<uint16_t*>(value ? c.v : c.k) + h * (value ? c.v_head : c.k_head) + x;
+      const int64_t block = value ? c.v_block : c.k_block, token = value ? c.v_token : c.k_token;
+      for (int r = 0; r < count; r += kCopyRows) {
+        uint4 held[kCopyRows];
+        bool there[kCopyRows];
 #pragma unroll
-    for (int i = 0; i < kCopyRows; ++i) {
-      if (head[i] >= 0) {
-        uint16_t* dst = static_cast<uint16_t*>(value ? c.v : c.k);
-        *reinterpret_cast<uint4*>(dst + place(to[i], head[i], value) + x) = held[i];
+        for (int i = 0; i < kCopyRows; ++i) {
+          const int page = __shfl_sync(0xffffffffu, from_page, (r + i) % kWarp);
+          const int off = __shfl_sync(0xffffffffu, from_off, (r + i) % kWarp);
+          there[i] = inside && page >= 0 && r + i < count;
+          if (there[i]) held[i] = ld_stream_v4(src + page * block + off * token);
+        }
+#pragma unroll
+        for (int i = 0; i < kCopyRows; ++i) {
+          const int page = __shfl_sync(0xffffffffu, to_page, (r + i) % kWarp);
+          const int off = __shfl_sync(0xffffffffu, to_off, (r + i) % kWarp);
+          if (there[i]) *reinterpret_cast<uint4*>(dst + page * block + off * token) = held[i];
+        }
       }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kCopyRows; ++i) {
-    if (lane == i && head[i] >= 0) {
-      auto weight = [&](const Slot& s) -> float& {
-        return c.weights[(static_cast<int64_t>(s.page) * c.hkv + head[i]) * c.block_size + s.offset];
-      };
-      weight(to[i]) = weight(from[i]);
     }
   }
 }
@@ -224,6 +232,7 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   if (!status) return cudaErrorInitializationError;
   const int64_t most = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
   const int held = static_cast<int>(most < kHeldKeys ? most : kHeldKeys);
+  const Divider by_page(static_cast<uint32_t>(a.cache.block_size));
   static std::once_flag once[64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -234,15 +243,13 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   });
   if (err != cudaSuccess) return err;
   err = launch_serialised(evict_select_kernel, dim3(a.batch * a.cache.hkv), dim3(kSelectThreads),
-                          static_cast<size_t>(held) * 4, stream, 1, a, held, status);
+                          static_cast<size_t>(held) * 4, stream, 1, a, by_page, held, status);
   if (err != cudaSuccess) return err;
   const int64_t longest = a.budget < most ? a.budget : most;
-  const int64_t rows = longest * a.cache.hkv;
-  if (rows == 0) return cudaSuccess;
-  const int per = kCopyThreads / kWarp * kCopyRows;
+  if (longest == 0) return cudaSuccess;
   return launch_serialised(evict_copy_kernel,
-                           dim3(static_cast<unsigned>((rows + per - 1) / per), a.batch),
-                           dim3(kCopyThreads), 0, stream, 1, a, status);
+                           dim3(static_cast<unsigned>((longest + kWarp - 1) / kWarp), a.batch),
+                           dim3(kCopyThreads), 0, stream, 1, a, by_page, status);
 }
 
 }  // namespace i4
