@@ -17,7 +17,7 @@
 namespace i4 {
 namespace {
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / kWarp;
 constexpr int kBins = 2048;
 constexpr int kReads = 8;  // weights a thread has in flight
@@ -34,11 +34,28 @@ __device__ __forceinline__ int clamped_length(int n, int most, int* status) {
   return n;
 }
 
-__global__ void __launch_bounds__(kSelectThreads)
+// Sum of v over this thread and those before it. Ends with a barrier.
+__device__ __forceinline__ int block_prefix(int v, int* warp_sums) {
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+#pragma unroll
+  for (int off = 1; off < kWarp; off *= 2) {
+    const int o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  if (lane == kWarp - 1) warp_sums[warp] = v;
+  __syncthreads();
+  int before = lane < warp ? warp_sums[lane] : 0;
+#pragma unroll
+  for (int off = kWarp / 2; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
+  __syncthreads();
+  return v + before;
+}
+
+__global__ void __launch_bounds__(kSelectThreads, 3)
     evict_select_kernel(const PagedEvictArgs a, const Divider by_page, int held, int* status) {
   extern __shared__ uint32_t keys[];  // [held]
   __shared__ int bins[kBins];
-  __shared__ int warp_gt[kSelectWarps], warp_eq[kSelectWarps], found_bin, found_above;
+  __shared__ int warp_sums[kSelectWarps], found_bin, found_above;
   wait_then_release();
   const int hkv = a.cache.hkv, page = a.cache.block_size;
   const int b = blockIdx.x / hkv, head = blockIdx.x % hkv;
@@ -98,24 +115,23 @@ __global__ void __launch_bounds__(kSelectThreads)
       if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1);
     }
     __syncthreads();
-    // thread t owns bins 2 t and 2 t + 1 counted from the top; the sum of all bins above them
-    const int hi = kBins - 1 - 2 * tid;
-    const int own = bins[hi] + bins[hi - 1];
-    int upto = own;
+    // thread t owns the bins t kOwn ... counted from the top; `above`: the keys in bins above them
+    constexpr int kOwn = kBins / kSelectThreads;
+    const int hi = kBins - 1 - kOwn * tid;
+    int own = 0;
 #pragma unroll
-    for (int off = 1; off < kWarp; off *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += v;
-    }
-    if (lane == kWarp - 1) warp_gt[warp] = upto;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += warp_gt[w];
-    const int above = before + upto - own;  // keys in bins above this thread's
+    for (int i = 0; i < kOwn; ++i) own += bins[hi - i];
+    int above = block_prefix(own, warp_sums) - own;
     if (above < left && left <= above + own) {
-      const bool first = left <= above + bins[hi];
-      found_bin = first ? hi : hi - 1;
-      found_above = first ? above : above + bins[hi];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int here = bins[hi - i];
+        if (above < left && left <= above + here) {
+          found_bin = hi - i;
+          found_above = above;
+        }
+        above += here;
+      }
     }
     __syncthreads();
     left -= found_above;
@@ -134,16 +150,10 @@ __global__ void __launch_bounds__(kSelectThreads)
     gt += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k > least));
     eq += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k == least));
   }
-  if (lane == 0) {
-    warp_gt[warp] = gt;
-    warp_eq[warp] = eq;
-  }
-  __syncthreads();
-  int at = 0, eq_at = 0;
-  for (int w = 0; w < warp; ++w) {
-    at += warp_gt[w];
-    eq_at += warp_eq[w];
-  }
+  // positions above `least` and equal to it before this warp's range
+  const int gt_upto = block_prefix(lane == 0 ? gt : 0, warp_sums);
+  const int eq_upto = block_prefix(lane == 0 ? eq : 0, warp_sums);
+  int at = __shfl_sync(0xffffffffu, gt_upto, 0) - gt, eq_at = __shfl_sync(0xffffffffu, eq_upto, 0) - eq;
   const uint32_t below = (1u << lane) - 1;
   for (int j = j0; j < j1; j += kWarp) {
     const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
@@ -159,24 +169,26 @@ __global__ void __launch_bounds__(kSelectThreads)
 
 constexpr int kCopyThreads = 256;
 constexpr int kCopyWarps = kCopyThreads / kWarp;
-constexpr int kCopyRows = 8;  // positions a warp has in flight
+constexpr int kDepth = 16;  // 16-byte pieces a lane has in flight
+constexpr int kCopySmem = kCopyWarps * kDepth * kWarp * 16;
 
+// `span` positions a warp, at most 32.
 __global__ void __launch_bounds__(kCopyThreads)
-    evict_copy_kernel(const PagedEvictArgs a, const Divider by_page, int* status) {
+    evict_copy_kernel(const PagedEvictArgs a, const Divider by_page, int span, int* status) {
+  extern __shared__ __align__(16) unsigned char ring_raw[];
   wait_then_release();
   const PagedCache& c = a.cache;
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int b = blockIdx.y;
   const int kept = a.new_lens[b];
-  const int j0 = blockIdx.x * kWarp;
+  const int j0 = blockIdx.x * span;
   if (j0 >= kept) return;
   const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
   const int* new_table = a.new_table + static_cast<int64_t>(b) * a.new_blocks;
-  // elements are moved as 16-bit words of either type
-  const uint16_t* k = static_cast<const uint16_t*>(c.k);
-  const uint16_t* v = static_cast<const uint16_t*>(c.v);
   const int vectors = c.dim / 8;  // 16-byte pieces of a row of keys
-  const int count = min(kWarp, kept - j0);
+  const int parts = (2 * vectors + kWarp - 1) / kWarp;  // a position's key and value, a piece a lane
+  const int count = min(span, kept - j0);
+  const uint32_t ring = smem_addr(ring_raw) + (warp * kDepth * kWarp + lane) * 16;
 
   for (int h = warp; h < c.hkv; h += kCopyWarps) {
     // this lane's position: where it is and where it goes
@@ -198,29 +210,35 @@ __global__ void __launch_bounds__(kCopyThreads)
             c.weights[(static_cast<int64_t>(from_page) * c.hkv + h) * c.block_size + from_off];
       }
     }
-    for (int i0 = lane; i0 < 2 * vectors + lane; i0 += kWarp) {  // all lanes take part in the shuffles
-      const bool inside = i0 < 2 * vectors, value = i0 >= vectors;
-      const int x = (value ? i0 - vectors : i0) * 8;
-      const uint16_t* src = (value ? v : k) + h * (value ? c.v_head : c.k_head) + x;
-      uint16_t* dst = static_cast<uint16_t*>(value ? c.v : c.k) + h * (value ? c.v_head : c.k_head) + x;
+    for (int part = 0; part < parts; ++part) {
+      const int piece = part * kWarp + lane;
+      const bool value = piece >= vectors;
+      const int64_t x = (value ? piece - vectors : piece) * 8 + h * (value ? c.v_head : c.k_head);
+      uint16_t* cache = static_cast<uint16_t*>(value ? c.v : c.k) + x;  // 16-bit words of either type
       const int64_t block = value ? c.v_block : c.k_block, token = value ? c.v_token : c.k_token;
-      for (int r = 0; r < count; r += kCopyRows) {
-        uint4 held[kCopyRows];
-        bool there[kCopyRows];
-#pragma unroll
-        for (int i = 0; i < kCopyRows; ++i) {
-          const int page = __shfl_sync(0xffffffffu, from_page, (r + i) % kWarp);
-          const int off = __shfl_sync(0xffffffffu, from_off, (r + i) % kWarp);
-          there[i] = inside && page >= 0 && r + i < count;
-          if (there[i]) held[i] = ld_stream_v4(src + page * block + off * token);
+      auto read = [&](int r) {
+        const int page = __shfl_sync(0xffffffffu, from_page, r % kWarp);
+        const int off = __shfl_sync(0xffffffffu, from_off, r % kWarp);
+        if (r < count && page >= 0 && piece < 2 * vectors) {
+          cp_async_16(ring + r % kDepth * kWarp * 16, cache + page * block + off * token);
         }
-#pragma unroll
-        for (int i = 0; i < kCopyRows; ++i) {
-          const int page = __shfl_sync(0xffffffffu, to_page, (r + i) % kWarp);
-          const int off = __shfl_sync(0xffffffffu, to_off, (r + i) % kWarp);
-          if (there[i]) *reinterpret_cast<uint4*>(dst + page * block + off * token) = held[i];
+        cp_async_commit();
+      };
+#pragma unroll 4
+      for (int r = 0; r < kDepth; ++r) read(r);
+#pragma unroll 4
+      for (int r = 0; r < count; ++r) {
+        cp_async_wait<kDepth - 1>();
+        const uint4 held = ld_shared_v4(ring + r % kDepth * kWarp * 16);
+        const bool there = __shfl_sync(0xffffffffu, from_page, r) >= 0;
+        const int page = __shfl_sync(0xffffffffu, to_page, r);
+        const int off = __shfl_sync(0xffffffffu, to_off, r);
+        if (there && piece < 2 * vectors) {
+          *reinterpret_cast<uint4*>(cache + page * block + off * token) = held;
         }
+        read(r + kDepth);
       }
+      cp_async_wait<0>();  // empty groups; the ring starts anew
     }
   }
 }
@@ -240,6 +258,9 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   std::call_once(once[dev & 63], [&] {
     err = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kHeldKeys * 4);
+    if (err != cudaSuccess) return;
+    err = cudaFuncSetAttribute(evict_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kCopySmem);
   });
   if (err != cudaSuccess) return err;
   err = launch_serialised(evict_select_kernel, dim3(a.batch * a.cache.hkv), dim3(kSelectThreads),
@@ -247,9 +268,12 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const int64_t longest = a.budget < most ? a.budget : most;
   if (longest == 0) return cudaSuccess;
+  // 32 positions a warp where that gives every SM three blocks, down to 8 where it does not
+  int span = kWarp;
+  while (span > 8 && (longest + span - 1) / span * a.batch < 3 * sm_count()) span /= 2;
   return launch_serialised(evict_copy_kernel,
-                           dim3(static_cast<unsigned>((longest + kWarp - 1) / kWarp), a.batch),
-                           dim3(kCopyThreads), 0, stream, 1, a, by_page, status);
+                           dim3(static_cast<unsigned>((longest + span - 1) / span), a.batch),
+                           dim3(kCopyThreads), kCopySmem, stream, 1, a, by_page, span, status);
 }
 
 }  // namespace i4
