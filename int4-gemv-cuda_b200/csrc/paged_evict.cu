@@ -9,6 +9,7 @@
 // a position. The copy: a warp a (position, head), 16 bytes a lane, bound by HBM. The new pages are
 // not the old ones, so every block of the copy is independent of the others and sequences may
 // share old pages (a common prefix).
+#include <algorithm>
 #include <mutex>
 
 #include "decode.cuh"
@@ -20,7 +21,6 @@ namespace {
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / kWarp;
 constexpr int kBins = 2048;
-constexpr int kReads = 8;  // weights a thread has in flight
 constexpr int kHeldKeys = 48 * 1024;  // weights kept in shared memory; longer ones are read again
 
 __device__ __forceinline__ void bad_page(int* status) { atomicExch(status, kStatusBadPage); }
@@ -34,28 +34,31 @@ __device__ __forceinline__ int clamped_length(int n, int most, int* status) {
   return n;
 }
 
-// Sum of v over this thread and those before it. Ends with a barrier.
-__device__ __forceinline__ int block_prefix(int v, int* warp_sums) {
+// Sum of v over this thread and those before it, behind a barrier.
+template <class V>
+__device__ __forceinline__ V block_prefix(V v, V* warp_sums) {
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
 #pragma unroll
   for (int off = 1; off < kWarp; off *= 2) {
-    const int o = __shfl_up_sync(0xffffffffu, v, off);
+    const V o = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= off) v += o;
   }
   if (lane == kWarp - 1) warp_sums[warp] = v;
   __syncthreads();
-  int before = lane < warp ? warp_sums[lane] : 0;
+  V before = lane < warp ? warp_sums[lane] : 0;
 #pragma unroll
-  for (int off = kWarp / 2; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
-  __syncthreads();
-  return v + before;
+  for (int off = kSelectWarps / 2; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
+  return v + __shfl_sync(0xffffffffu, before, 0);
 }
 
+// kFour: pages of a multiple of four positions, whose weights are read four at a time.
+template <bool kFour>
 __global__ void __launch_bounds__(kSelectThreads, 3)
     evict_select_kernel(const PagedEvictArgs a, const Divider by_page, int held, int* status) {
-  extern __shared__ uint32_t keys[];  // [held]
+  extern __shared__ __align__(16) uint32_t keys[];  // [held], held a multiple of four
   __shared__ int bins[kBins];
   __shared__ int warp_sums[kSelectWarps], found_bin, found_above;
+  __shared__ unsigned long long warp_pairs[kSelectWarps];
   wait_then_release();
   const int hkv = a.cache.hkv, page = a.cache.block_size;
   const int b = blockIdx.x / hkv, head = blockIdx.x % hkv;
@@ -78,87 +81,130 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
   if (want == 0) return;
 
   const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
-  auto read_key = [&](int j) -> uint32_t {
+  // the weight of position j, or null
+  auto weight_at = [&](int j) -> const float* {
     const int block = by_page.quotient(j), p = table[block];
     if (static_cast<unsigned>(p) >= static_cast<unsigned>(a.cache.num_blocks)) {
       bad_page(status);
-      return 0;
+      return nullptr;
     }
-    return order_key(a.cache.weights[(static_cast<int64_t>(p) * hkv + head) * page + j - block * page]);
+    return a.cache.weights + (static_cast<int64_t>(p) * hkv + head) * page + (j - block * page);
   };
-  for (int j0 = tid; j0 < min(old, held); j0 += kReads * kSelectThreads) {
-    uint32_t k[kReads];  // kept apart from the stores, so that the reads do not wait for each other
+  auto read_key = [&](int j) -> uint32_t {
+    const float* w = weight_at(j);
+    return w ? order_key(*w) : 0;
+  };
+  const int here = min(old, held);  // keys kept in shared memory
+  if constexpr (kFour) {
+    constexpr int kAtOnce = 2;
+    for (int j0 = tid * 4; j0 < here; j0 += kAtOnce * kSelectThreads * 4) {
+      float4 w[kAtOnce];
+      bool there[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < kReads; ++i) {
-      const int j = j0 + i * kSelectThreads;
-      k[i] = j < min(old, held) ? read_key(j) : 0;
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kSelectThreads * 4;
+        const float* from = j < here ? weight_at(j) : nullptr;
+        there[i] = from != nullptr;
+        if (there[i]) w[i] = *reinterpret_cast<const float4*>(from);
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kSelectThreads * 4;
+        if (j < here) {  // up to the next multiple of four, which held is
+          *reinterpret_cast<uint4*>(&keys[j]) =
+              there[i] ? make_uint4(order_key(w[i].x), order_key(w[i].y), order_key(w[i].z),
+                                    order_key(w[i].w))
+                       : make_uint4(0, 0, 0, 0);
+        }
+      }
     }
+  } else {
+    constexpr int kAtOnce = 8;
+    for (int j0 = tid; j0 < here; j0 += kAtOnce * kSelectThreads) {
+      uint32_t k[kAtOnce];  // kept apart from the stores, so that the reads do not wait for each other
 #pragma unroll
-    for (int i = 0; i < kReads; ++i) {
-      const int j = j0 + i * kSelectThreads;
-      if (j < min(old, held)) keys[j] = k[i];
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kSelectThreads;
+        k[i] = j < here ? read_key(j) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int j = j0 + i * kSelectThreads;
+        if (j < here) keys[j] = k[i];
+      }
     }
   }
-  auto key = [&](int j) { return j < held ? keys[j] : read_key(j); };
 
   // the want-th largest key, digit by digit
+  constexpr int kOwn = kBins / kSelectThreads;
+  const int hi = kBins - 1 - kOwn * tid;  // this thread's bins, counted from the top
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) bins[hi - i] = 0;
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int left = want;  // rank still to find among the keys that match the prefix
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int width = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < old; j += kSelectThreads) {
-      const uint32_t k = key(j);
-      if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1);
+    const uint32_t digit = pass == 2 ? 0x3FF : 0x7FF;
+#pragma unroll 4
+    for (int j = tid; j < here; j += kSelectThreads) {
+      const uint32_t k = keys[j];
+      if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & digit], 1);
+    }
+    for (int j = here + tid; j < old; j += kSelectThreads) {
+      const uint32_t k = read_key(j);
+      if ((k & mask) == prefix) atomicAdd(&bins[(k >> shift) & digit], 1);
     }
     __syncthreads();
-    // thread t owns the bins t kOwn ... counted from the top; `above`: the keys in bins above them
-    constexpr int kOwn = kBins / kSelectThreads;
-    const int hi = kBins - 1 - kOwn * tid;
-    int own = 0;
+    int own[kOwn], sum = 0;
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) own += bins[hi - i];
-    int above = block_prefix(own, warp_sums) - own;
-    if (above < left && left <= above + own) {
+    for (int i = 0; i < kOwn; ++i) {
+      own[i] = bins[hi - i];
+      bins[hi - i] = 0;  // for the next pass
+      sum += own[i];
+    }
+    int above = block_prefix(sum, warp_sums) - sum;  // keys in the bins above this thread's
+    if (above < left && left <= above + sum) {
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
-        const int here = bins[hi - i];
-        if (above < left && left <= above + here) {
+        if (above < left && left <= above + own[i]) {
           found_bin = hi - i;
           found_above = above;
         }
-        above += here;
+        above += own[i];
       }
     }
     __syncthreads();
     left -= found_above;
     prefix |= static_cast<uint32_t>(found_bin) << shift;
-    mask |= ((1u << width) - 1) << shift;
-    __syncthreads();
+    mask |= digit << shift;
+    // found_* and warp_sums are written again behind the next pass's barrier
   }
   const uint32_t least = prefix;  // keys above it stay, and the first `left` of those equal to it
 
   // each warp owns a contiguous range, so ranks follow from counts of the warps before it
+  auto key = [&](int j) { return j < held ? keys[j] : read_key(j); };
   const int range = ((old + kSelectWarps - 1) / kSelectWarps + kWarp - 1) / kWarp * kWarp;
   const int j0 = min(warp * range, old), j1 = min(j0 + range, old);
-  int gt = 0, eq = 0;
-  for (int j = j0; j < j1; j += kWarp) {
-    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
-    gt += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k > least));
-    eq += __popc(__ballot_sync(0xffffffffu, j + lane < j1 && k == least));
+  int gt = 0, eq = 0;  // of this lane
+#pragma unroll 4
+  for (int j = j0 + lane; j < j1; j += kWarp) {
+    const uint32_t k = key(j);
+    gt += k > least;
+    eq += k == least;
   }
-  // positions above `least` and equal to it before this warp's range
-  const int gt_upto = block_prefix(lane == 0 ? gt : 0, warp_sums);
-  const int eq_upto = block_prefix(lane == 0 ? eq : 0, warp_sums);
-  int at = __shfl_sync(0xffffffffu, gt_upto, 0) - gt, eq_at = __shfl_sync(0xffffffffu, eq_upto, 0) - eq;
+  // both counts in one number: positions above `least` and equal to it before this warp's range
+  const unsigned long long pair = static_cast<unsigned long long>(eq) << 32 | static_cast<uint32_t>(gt);
+  const unsigned long long upto = block_prefix(pair, warp_pairs);
+  const unsigned long long start = __shfl_sync(0xffffffffu, upto - pair, 0);
+  int at = static_cast<int>(static_cast<uint32_t>(start)), eq_at = static_cast<int>(start >> 32);
   const uint32_t below = (1u << lane) - 1;
   for (int j = j0; j < j1; j += kWarp) {
-    const uint32_t k = j + lane < j1 ? key(j + lane) : 0;
-    const uint32_t gts = __ballot_sync(0xffffffffu, j + lane < j1 && k > least);
-    const uint32_t eqs = __ballot_sync(0xffffffffu, j + lane < j1 && k == least);
+    const bool inside = j + lane < j1;
+    const uint32_t k = inside ? key(j + lane) : 0;
+    const uint32_t gts = __ballot_sync(0xffffffffu, inside && k > least);
+    const uint32_t eqs = __ballot_sync(0xffffffffu, inside && k == least);
     const int my_eq = eq_at + __popc(eqs & below);
     const bool stays = (gts >> lane & 1) || ((eqs >> lane & 1) && my_eq < left);
     if (stays) out[at + __popc(gts & below) + min(my_eq, left)] = j + lane;
@@ -249,21 +295,23 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   int* status = device_status_word();
   if (!status) return cudaErrorInitializationError;
   const int64_t most = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
-  const int held = static_cast<int>(most < kHeldKeys ? most : kHeldKeys);
+  const int held = static_cast<int>(std::min<int64_t>((most + 3) / 4 * 4, kHeldKeys));
+  const bool four = a.cache.block_size % 4 == 0 && reinterpret_cast<uintptr_t>(a.cache.weights) % 16 == 0;
+  const auto select = four ? evict_select_kernel<true> : evict_select_kernel<false>;
   const Divider by_page(static_cast<uint32_t>(a.cache.block_size));
-  static std::once_flag once[64];
+  static std::once_flag once[2][64];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  std::call_once(once[dev & 63], [&] {
-    err = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  std::call_once(once[four][dev & 63], [&] {
+    err = cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kHeldKeys * 4);
     if (err != cudaSuccess) return;
     err = cudaFuncSetAttribute(evict_copy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kCopySmem);
   });
   if (err != cudaSuccess) return err;
-  err = launch_serialised(evict_select_kernel, dim3(a.batch * a.cache.hkv), dim3(kSelectThreads),
+  err = launch_serialised(select, dim3(a.batch * a.cache.hkv), dim3(kSelectThreads),
                           static_cast<size_t>(held) * 4, stream, 1, a, by_page, held, status);
   if (err != cudaSuccess) return err;
   const int64_t longest = a.budget < most ? a.budget : most;
