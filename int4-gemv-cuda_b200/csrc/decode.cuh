@@ -14,8 +14,9 @@ namespace i4 {
 // then let the next one launch. In this order a kernel that starts early (this library's GEMVs
 // fetch their weights before their own wait) has everything before this kernel complete and
 // visible, so weights written by a kernel that was followed by one of these are safe to prefetch.
+__device__ __forceinline__ void wait_only() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void wait_then_release() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_only();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 

@@ -40,13 +40,16 @@ struct Shape {
   static constexpr int kWarps = DP == 256 ? 6 : 4;
   static constexpr int kThreads = kWarps * kWarp;
   static constexpr int kTile = kWarps * kWarpTile;
+  // Ring stages and blocks an SM: what fits the shared memory, measured against its neighbours. At
+  // 128 dims 3 blocks x 2 stages, against 2 x 3: sequences of 512 to 8192 positions, 64 of them, 198
+  // against 225 us (the more blocks, the less the end of a segment shows), 131072 positions 99
+  // against 97 us.
   static constexpr int kStages = DP == 64 ? 3 : 2;
-  static constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? (NT == 1 ? 3 : 2) : 1;  // of an SM
+  static constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? (NT == 1 ? 3 : 2) : 1;
   static constexpr int kChunks = DP / 8;                // 16-byte chunks of a row
   static constexpr int kPitch = DP * 2 + 16;            // of a row in shared memory: the eight rows
                                                         // of an ldmatrix fall into different banks
   static constexpr int kHalf = kWarpTile * kPitch;      // K or V of a warp's tile
-  static constexpr bool kHoldQ = DP * NT <= 256;        // in registers; else in shared memory
 };
 constexpr int round_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -59,6 +62,8 @@ struct Plan {
   int tile;        // positions of a tile
   int blocks;      // blocks of the attention kernel
   int max_len;     // positions the table has room for
+  int join_warps;   // of a head in the joining kernel
+  int join_blocks;  // of that kernel, for the heads
   int score_rows;  // heads of an item rounded up to a pair
   Divider page;
   float* part_o;    // [2 blocks][rows][dim]: the segments of items that a block shares
@@ -148,7 +153,6 @@ template <int DP, int NT>
 struct Smem {
   using S = Shape<DP, NT>;
   alignas(128) unsigned char ring[S::kWarps][S::kStages][2][S::kHalf];
-  alignas(16) unsigned char q[S::kHoldQ ? 16 : S::kRows * S::kPitch];
   const void* rows[S::kWarps][kWarpTile][2];  // K and V row of each position of the tile being loaded
   uint32_t mask[S::kWarps][S::kStages];       // positions that count
   float joined[S::kRows][DP];
@@ -164,7 +168,9 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
   constexpr int kTile = S::kTile, kThreads = S::kThreads, kWarps = S::kWarps;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Smem<DP, NT>& sh = *reinterpret_cast<Smem<DP, NT>*>(smem_raw);
-  wait_then_release();
+  // The joining kernel starts when this one has left: its blocks, waiting beside these, made the next
+  // call's start late (16 x 8192 positions of 8 heads: 130 us, against 101 without).
+  wait_only();
   const PagedAttentionArgs& a = p.a;
   const PagedCache& c = a.cache;
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
@@ -326,39 +332,28 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
 
   // ---- computing
   const int g = lane / 4, t2 = lane % 4 * 2;
-  uint32_t qf[S::kHoldQ ? DP / 16 : 1][NT][2];
+  uint32_t qf[DP / 16][NT][2];
   float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
   float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the maximum of all lanes, this lane's sum
-  auto begin = [&] {
-    const int kv = now.item / p.head_tiles, h0 = now.item % p.head_tiles * S::kRows;
+  auto load_q = [&](const Walker& at) {
+    const int kv = at.item / p.head_tiles, h0 = at.item % p.head_tiles * S::kRows;
     const T* q = static_cast<const T*>(a.q) +
-                 (static_cast<int64_t>(now.b) * a.hq + kv * p.group + h0) * c.dim;
-    if constexpr (S::kHoldQ) {
+                 (static_cast<int64_t>(at.b) * a.hq + kv * p.group + h0) * c.dim;
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
+    for (int k = 0; k < DP / 16; ++k) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
+      for (int i = 0; i < NT; ++i) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int row = i * 8 + g, col = k * 16 + j * 8 + t2;
-            qf[k][i][j] = h0 + row < p.group && col < c.dim
-                              ? *reinterpret_cast<const uint32_t*>(q + row * c.dim + col)
-                              : 0u;
-          }
+        for (int j = 0; j < 2; ++j) {
+          const int row = i * 8 + g, col = k * 16 + j * 8 + t2;
+          qf[k][i][j] = h0 + row < p.group && col < c.dim
+                            ? *reinterpret_cast<const uint32_t*>(q + row * c.dim + col)
+                            : 0u;
         }
       }
-    } else {
-      // every warp is past its use of the segment before (the join's barriers)
-      for (int i = tid; i < S::kRows * S::kChunks; i += kThreads) {
-        const int row = i / S::kChunks, chunk = i % S::kChunks;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (h0 + row < p.group && chunk * 8 < c.dim) {
-          v = *reinterpret_cast<const uint4*>(q + row * c.dim + chunk * 8);
-        }
-        *reinterpret_cast<uint4*>(sh.q + row * S::kPitch + chunk * 16) = v;
-      }
-      __syncthreads();
     }
+  };
+  auto begin = [&] {
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
 #pragma unroll
@@ -370,6 +365,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
       l[j][0] = l[j][1] = 0.0f;
     }
   };
+  load_q(now);
   begin();
   // the lanes' rows and chunks in the ldmatrix of K (positions 0-7, 8-15 by k 0-7, then by 8-15)
   // and of V (positions 0-7 by dims 0-7, by 8-15, then positions 8-15)
@@ -383,6 +379,9 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
     const uint32_t tile = ring + stage * 2 * S::kHalf;
     const uint32_t mask = sh.mask[warp][stage];
     load_next();
+    const bool item_ends = now.tile + 1 == now.tiles;
+    Walker following = now;
+    if (item_ends && t + 1 < t1) following.template next<kTile>(p);
 
     if (mask != 0 || kWeights) {
       // S^T: positions g, g + 8 by heads t2, t2 + 1
@@ -392,17 +391,8 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
         if (k * 16 < c.dim) {
           uint32_t f[4];
           ldmatrix_x4(f, tile + k_lane + k * 32);
-          if constexpr (S::kHoldQ) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) mma<T>(s[i], f, qf[k][i][0], qf[k][i][1]);
-          } else {
-            static_assert(S::kHoldQ || NT == 2, "an ldmatrix brings two blocks of heads");
-            uint32_t b[4];  // heads 0-7 by k 0-7, by 8-15, then heads 8-15
-            ldmatrix_x4(b, smem_addr(sh.q) + ((lane & 7) + (lane >> 4) * 8) * S::kPitch +
-                               (lane >> 3 & 1) * 16 + k * 32);
-            mma<T>(s[0], f, b[0], b[1]);
-            mma<T>(s[NT - 1], f, b[2], b[3]);
-          }
+          for (int i = 0; i < NT; ++i) mma<T>(s[i], f, qf[k][i][0], qf[k][i][1]);
         }
       }
 #pragma unroll
@@ -410,6 +400,8 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] *= a.scale_log2;
       }
+      // the next item's queries are on their way while this one is finished
+      if (item_ends && t + 1 < t1) load_q(following);
       if (mask != 0xFFFFu) {
         const bool at[2] = {(mask >> g & 1) != 0, (mask >> (g + 8) & 1) != 0};
 #pragma unroll
@@ -489,11 +481,11 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
         }
       }
     }
+    if (mask == 0 && !kWeights && item_ends && t + 1 < t1) load_q(following);
     __syncwarp();  // this stage is refilled by the next load_next
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
     // ---- the end of a segment: join the warps
-    const bool item_ends = now.tile + 1 == now.tiles;
     if (!item_ends && t + 1 < t1) {
       ++now.tile;
       continue;
@@ -527,17 +519,21 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
         f[i][j] = m[i][j] == -INFINITY ? 1.0f : exp2_fast(m[i][j] - top);
       }
     }
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) {
+    // the warps add their sums to one place in rounds, each to another share of the dimensions, so
+    // the order at every place is fixed and no warp waits for its turn
+#pragma unroll 1
+    for (int round = 0; round < kWarps; ++round) {
+      const int share = (warp + round) % kWarps;
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
+      for (int d = 0; d < DP / 16; ++d) {
+        if (d % kWarps == share) {
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               float* to = &sh.joined[i * 8 + t2 + (j & 1)][d * 16 + g + j / 2 * 8];
               const float v = o[d][i][j] * f[i][j & 1];
-              *to = w == 0 ? v : *to + v;
+              *to = round == 0 ? v : *to + v;
             }
           }
         }
@@ -579,7 +575,7 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
     }
     __syncthreads();  // joined and ml are written again by the next segment
     if (t + 1 < t1) {
-      now.next<kTile>(p);
+      now = following;
       segment = t + 1;
       begin();
     }
@@ -588,10 +584,11 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
 
 // ---- Joining -------------------------------------------------------------------------------------
 //
-// A block a (sequence, query head) joins what several blocks of the attention kernel hold of it:
-// the warps take the parts in turn, a lane four dimensions at a time, then the warps' sums are
-// added. It also zeroes the output of empty sequences. Blocks behind those add the weights: an even
-// share of the tiles each, a thread a position.
+// A warp a (sequence, query head), or a block where items have many parts, joins what several blocks
+// of the attention kernel hold of it: a lane takes four dimensions of part after part, a block's warps
+// take the parts in turn and their sums are added in order. It also zeroes the output of empty
+// sequences. Blocks behind those add the weights: an even share of the tiles each, a thread two
+// positions at a time.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / kWarp;
 constexpr int kMaxDim = 256;
@@ -627,50 +624,91 @@ struct Parts {
 };
 
 template <class T>
-__device__ __forceinline__ void join_head(const Plan& p, int index) {
+__device__ __forceinline__ void join_head(const Plan& p) {
   __shared__ alignas(16) float sums[kJoinWarps][kMaxDim];
   const PagedAttentionArgs& a = p.a;
-  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp, dim = a.cache.dim;
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp, dim = a.cache.dim;
+  const int index = p.join_warps == 1 ? blockIdx.x * kJoinWarps + warp : blockIdx.x;
+  const int sub = p.join_warps == 1 ? 0 : warp;
+  if (index >= a.batch * a.hq) return;
   const int b = index / a.hq, head = index % a.hq;
   const int kv = head / p.group, h = head % p.group;
   const int item = kv * p.head_tiles + h / p.rows, row = h % p.rows;
   const int first = p.first_tile[b], tiles = (p.first_tile[b + 1] - first) / p.items;
   T* out = static_cast<T*>(a.out) + static_cast<int64_t>(index) * dim;
   if (tiles == 0) {
-    for (int i = tid; i < dim; i += kJoinThreads) out[i] = from_f32<T>(0.0f);
+    if (sub == 0) {
+      for (int i = lane; i < dim; i += kWarp) out[i] = from_f32<T>(0.0f);
+    }
     return;
   }
   const Parts parts(p, p.first_tile[a.batch], first + item * tiles, tiles);
   if (parts.count == 1) return;
-  const float2 ml = parts.row(row, lane);
+  constexpr int kAtOnce = 4;
+  float2 ml = make_float2(0.0f, 0.0f);
   float4 v[2] = {};
-#pragma unroll 4
-  for (int i = warp; i < parts.count; i += kJoinWarps) {
-    const int64_t at = parts.slot(i) * p.rows + row;
-    const float f = Parts::factor(p.part_ml[at].x, ml.x);
+  for (int i0 = sub; i0 < parts.count; i0 += kAtOnce * p.join_warps) {
+    float m[kAtOnce];
+    float4 o[kAtOnce][2];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = i0 + k * p.join_warps;
+      if (i < parts.count) {
+        const int64_t at = parts.slot(i) * p.rows + row;
+        m[k] = p.part_ml[at].x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = (j * kWarp + lane) * 4;
+          if (d < dim) o[k][j] = *reinterpret_cast<const float4*>(p.part_o + at * dim + d);
+        }
+      }
+    }
+    if (i0 == sub) ml = parts.row(row, lane);  // while the first parts are on their way
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (i0 + k * p.join_warps >= parts.count) continue;
+      const float f = Parts::factor(m[k], ml.x);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if ((j * kWarp + lane) * 4 < dim) {
+          v[j].x = fmaf(o[k][j].x, f, v[j].x);
+          v[j].y = fmaf(o[k][j].y, f, v[j].y);
+          v[j].z = fmaf(o[k][j].z, f, v[j].z);
+          v[j].w = fmaf(o[k][j].w, f, v[j].w);
+        }
+      }
+    }
+  }
+  if (p.join_warps > 1) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int d = (j * kWarp + lane) * 4;
+      if (d < dim) *reinterpret_cast<float4*>(&sums[warp][d]) = v[j];
+    }
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int d = (j * kWarp + lane) * 4;
       if (d < dim) {
-        const float4 o = *reinterpret_cast<const float4*>(p.part_o + at * dim + d);
-        v[j].x = fmaf(o.x, f, v[j].x);
-        v[j].y = fmaf(o.y, f, v[j].y);
-        v[j].z = fmaf(o.z, f, v[j].z);
-        v[j].w = fmaf(o.w, f, v[j].w);
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) {
+          const float4 o = *reinterpret_cast<const float4*>(&sums[w][d]);
+          v[j].x += o.x;
+          v[j].y += o.y;
+          v[j].z += o.z;
+          v[j].w += o.w;
+        }
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int d = (j * kWarp + lane) * 4;
-    if (d < dim) *reinterpret_cast<float4*>(&sums[warp][d]) = v[j];
-  }
-  __syncthreads();
-  for (int d = tid; d < dim; d += kJoinThreads) {
-    float sum = sums[0][d];
-#pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) sum += sums[w][d];
-    out[d] = from_f32<T>(sum / ml.y);
+    if (d < dim) {
+      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[j].x / ml.y, v[j].y / ml.y),
+                                                      pack2<T>(v[j].z / ml.y, v[j].w / ml.y));
+    }
   }
 }
 
@@ -712,24 +750,37 @@ __device__ __forceinline__ void add_weights(const Plan& p, int block, int blocks
         }
       }
       __syncthreads();
-      for (int i = tid; i < count * p.tile; i += kJoinThreads) {
-        const int pos = tile0 * p.tile + i;
-        if (pos >= n) break;
-        const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + p.page.quotient(pos)];
-        const float2* s = reinterpret_cast<const float2*>(
-            p.scores + (static_cast<int64_t>(begin + tile0) * p.tile + i) * p.score_rows);
-        float w = 0.0f;
+      constexpr int kAtOnce = 2;
+      const int positions = min(count * p.tile, n - tile0 * p.tile);
+      for (int i0 = tid; i0 < positions; i0 += kAtOnce * kJoinThreads) {
+        float* to[kAtOnce];
+        float w[kAtOnce];
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int i = i0 + k * kJoinThreads, pos = tile0 * p.tile + i;
+          to[k] = nullptr;
+          w[k] = 0.0f;
+          if (i >= positions) continue;
+          const int block = p.page.quotient(pos);
+          const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + block];
+          const float2* s = reinterpret_cast<const float2*>(
+              p.scores + (static_cast<int64_t>(begin + tile0) * p.tile + i) * p.score_rows);
 #pragma unroll 4
-        for (int r = 0; r < rows; r += 2) {
-          const float2 v = s[r / 2];
-          w += exp2_fast(v.x - row_lse[r]);
-          if (r + 1 < rows) w += exp2_fast(v.y - row_lse[r + 1]);
+          for (int r = 0; r < rows; r += 2) {
+            const float2 v = s[r / 2];
+            w[k] += exp2_fast(v.x - row_lse[r]);
+            if (r + 1 < rows) w[k] += exp2_fast(v.y - row_lse[r + 1]);
+          }
+          if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
+            to[k] = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
+                    (pos - block * static_cast<int>(p.page.by));
+            // a new token's slot may hold what its page was used for before
+            if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] += *to[k];
+          }
         }
-        if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-          float* to = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
-                      (pos - p.page.quotient(pos) * p.page.by);
-          // a new token's slot may hold what its page was used for before
-          *to = ht == 0 && a.k_new && pos == n - 1 ? w : *to + w;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          if (to[k]) *to[k] = w[k];
         }
       }
       __syncthreads();  // row_lse is rewritten
@@ -741,11 +792,10 @@ __device__ __forceinline__ void add_weights(const Plan& p, int block, int blocks
 template <class T, bool kWeights>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Plan p) {
   wait_then_release();
-  const int heads = p.a.batch * p.a.hq;
-  if (static_cast<int>(blockIdx.x) < heads) {
-    join_head<T>(p, blockIdx.x);
+  if (static_cast<int>(blockIdx.x) < p.join_blocks) {
+    join_head<T>(p);
   } else if constexpr (kWeights) {
-    add_weights(p, blockIdx.x - heads, gridDim.x - heads);
+    add_weights(p, blockIdx.x - p.join_blocks, gridDim.x - p.join_blocks);
   }
 }
 
@@ -758,7 +808,7 @@ auto with_shape(int dim, int group, F f) {
   switch (round_dim(dim)) {
     case 64: return wide ? f.template operator()<64, 2>() : f.template operator()<64, 1>();
     case 128: return wide ? f.template operator()<128, 2>() : f.template operator()<128, 1>();
-    default: return wide ? f.template operator()<256, 2>() : f.template operator()<256, 1>();
+    default: return f.template operator()<256, 1>();  // 16 heads' sums do not fit the registers
   }
 }
 
@@ -788,6 +838,11 @@ int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
   p->page = Divider(static_cast<uint32_t>(a.cache.block_size));
   const int64_t resident = static_cast<int64_t>(sm_count()) * ctas;
   p->blocks = static_cast<int>(std::max<int64_t>(1, std::min(resident, tiles)));
+  // a block a head where an item has more than this many parts (1 x 131072 positions, 64 heads of 55
+  // parts; with few parts a warp leaves room for four times the heads)
+  constexpr int kManyParts = 6;
+  p->join_warps = p->blocks > kManyParts * a.batch * items ? kJoinWarps : 1;
+  p->join_blocks = (a.batch * a.hq * p->join_warps + kJoinWarps - 1) / kJoinWarps;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -818,10 +873,9 @@ cudaError_t launch(const Plan& p, cudaStream_t stream) {
   err = launch_serialised(paged_attention_kernel<T, DP, NT, kWeights>, dim3(p.blocks),
                           dim3(Shape<DP, NT>::kThreads), sizeof(Smem<DP, NT>), stream, 1, p);
   if (err != cudaSuccess) return err;
-  const int heads = p.a.batch * p.a.hq;
   return launch_serialised(paged_join_kernel<T, kWeights>,
-                           dim3(heads + (kWeights ? 4 * sm_count() : 0)), dim3(kJoinThreads), 0,
-                           stream, 1, p);
+                           dim3(p.join_blocks + (kWeights ? 8 * sm_count() : 0)),
+                           dim3(kJoinThreads), 0, stream, 1, p);
 }
 
 }  // namespace
