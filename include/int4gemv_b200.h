@@ -365,7 +365,7 @@ int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cach
                              int64_t q_heads, int64_t max_blocks, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
-/* Bytes of workspace for the current device, or -1 if the sizes are refused (see
+/* Bytes of workspace for the current device (0 where none is needed), or -1 if the sizes are refused (see
  * int4gemv_last_error). The pointers of `cache` are not used. */
 int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* cache, int64_t batch,
                                                 int64_t q_heads, int64_t max_blocks, int weights);

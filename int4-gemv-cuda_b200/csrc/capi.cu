@@ -342,7 +342,7 @@ int attention_sizes(const char* name, const int4gemv_paged_cache_t* c, int64_t b
   static float any;
   if (weights) a->cache.weights = &any;
   *bytes = i4::paged_attention_workspace_bytes(*a);
-  if (*bytes == 0) {
+  if (*bytes < 0) {
     return fail(INT4GEMV_ERR_INVALID,
                 "%s: batch = %lld with tables of %lld blocks of %lld is out of range", name,
                 static_cast<long long>(batch), static_cast<long long>(max_blocks),
@@ -1025,12 +1025,12 @@ int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cach
   if (!aligned_to(q, 16) || !aligned_to(out, 16) || !aligned_to(k_new, 16) || !aligned_to(v_new, 16)) {
     return fail(INT4GEMV_ERR_INVALID, "%s: q, out, k_new and v_new must be 16-byte aligned", name);
   }
-  if (!workspace || workspace_bytes < bytes || !aligned_to(workspace, 256)) {
+  if (bytes > 0 && (!workspace || workspace_bytes < bytes || !aligned_to(workspace, 256))) {
     return fail(INT4GEMV_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %lld bytes is needed, got %lld",
                 name, static_cast<long long>(bytes), static_cast<long long>(workspace ? workspace_bytes : 0));
   }
   // a flag for the kernel: weights are added where the pointer is set
-  if (add_weights && !some_pages) a.cache.weights = static_cast<float*>(workspace);
+  if (add_weights && !some_pages) a.cache.weights = reinterpret_cast<float*>(out);
   if (!some_pages) a.cache.k = a.cache.v = const_cast<void*>(q);  // an address that is not read
   a.out = out;
   a.q = q;

@@ -153,12 +153,13 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   const int64_t bytes = int4gemv_paged_attention_workspace_size(&cache, batch, q_heads, blocks, w != nullptr);
   TORCH_CHECK(bytes >= 0, int4gemv_last_error());
   at::Tensor out = at::empty(q.sizes(), q.options());
-  const at::Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  at::Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
   check_status(int4gemv_paged_attention(
       out.data_ptr(), q.data_ptr(), &cache, block_table.data_ptr<int>(), seq_lens.data_ptr<int>(),
       static_cast<float>(scale), k.has_value() ? k->data_ptr() : nullptr,
       v.has_value() ? v->data_ptr() : nullptr, w != nullptr, batch, q_heads, blocks,
-      workspace.data_ptr(), bytes, stream_of(q)));
+      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
   return out;
 }
 

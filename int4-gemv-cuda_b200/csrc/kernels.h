@@ -221,7 +221,7 @@ struct PagedAttentionArgs {
   float scale_log2;  // the scale of the scores times log2(e)
   void* workspace;
 };
-// Bytes of workspace a call needs; 0 if its sizes are out of the kernel's range.
+// Bytes of workspace a call needs (maybe 0); -1 if its sizes are out of the kernel's range.
 int64_t paged_attention_workspace_bytes(const PagedAttentionArgs& a);
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, int dtype, cudaStream_t stream);
 

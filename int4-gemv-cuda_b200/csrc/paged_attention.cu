@@ -12,6 +12,9 @@
 // block works through the end of one item, whole items, and the beginning of another; an item that
 // several blocks share is joined by a second kernel from partial sums in the workspace, in block
 // order (the same result every time, and no counters that a call would have to find cleared).
+// Small calls, whose time is mostly latency, give an item a cluster of blocks instead that join
+// through distributed shared memory: one kernel, no scan of the lengths, and nearly all of a block's
+// tiles on their way at once.
 //
 // A warp takes 16 positions of a tile and needs no other warp until its segment of an item ends:
 // it has its own ring of K and V tiles in shared memory, filled by cp.async (a row's page is looked
@@ -22,6 +25,8 @@
 // given to the MMA as a sum of two 16-bit numbers, so its rounding does not show in the result.
 // Positions behind the end are zero-filled in shared memory and masked, so nothing there reaches
 // a sum.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <mutex>
 
@@ -31,27 +36,37 @@
 namespace i4 {
 namespace {
 
-constexpr int kWarpTile = 16;  // positions a warp takes of a tile
+namespace cg = cooperative_groups;
 
-// What depends on the head dimension rounded up to DP and the heads of an item, 8 NT.
-template <int DP, int NT>
+constexpr int kWarpTile = 16;  // positions a warp takes of a tile
+constexpr int kMaxCluster = 8;
+constexpr int kMaxDim = 256;
+// A warp rescales its sums when a score passes their reference by this much (log2), not at every new
+// maximum: the factors stay at most 2^8, far inside of either 16-bit type.
+constexpr float kRise = 8.0f;
+
+// What depends on the head dimension rounded up to DP and the heads of an item, 8 NT; kSmall: the
+// kernel for small calls.
+template <int DP, int NT, bool kSmall>
 struct Shape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kWarps = DP == 256 ? 6 : 4;
+  static constexpr int kWarps = DP == 256 ? 6 : kSmall ? 8 : 4;
   static constexpr int kThreads = kWarps * kWarp;
   static constexpr int kTile = kWarps * kWarpTile;
-  // Ring stages and blocks an SM: what fits the shared memory, measured against its neighbours. At
-  // 128 dims 3 blocks x 2 stages, against 2 x 3: sequences of 512 to 8192 positions, 64 of them, 198
-  // against 225 us (the more blocks, the less the end of a segment shows), 131072 positions 99
-  // against 97 us.
-  static constexpr int kStages = DP == 64 ? 3 : 2;
-  static constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? (NT == 1 ? 3 : 2) : 1;
-  static constexpr int kChunks = DP / 8;                // 16-byte chunks of a row
-  static constexpr int kPitch = DP * 2 + 16;            // of a row in shared memory: the eight rows
-                                                        // of an ldmatrix fall into different banks
-  static constexpr int kHalf = kWarpTile * kPitch;      // K or V of a warp's tile
+  static constexpr int kStages = DP == 256 ? 2 : kSmall ? (DP == 64 ? 4 : 3) : DP == 64 ? 3 : 2;
+  static constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
+  static constexpr int kPitch = DP * 2 + 16;        // of a row in shared memory: the eight rows of
+                                                    // an ldmatrix fall into different banks
+  static constexpr int kHalf = kWarpTile * kPitch;  // K or V of a warp's tile
 };
+// Blocks an SM, and the ring stages above: what fits the shared memory, measured against its
+// neighbours. At 128 dims 3 blocks x 2 stages, against 2 x 3: sequences of 512 to 8192 positions, 64
+// of them, 198 against 225 us (the more blocks, the less the end of a segment shows), 131072
+// positions 99 against 97 us. Small calls have one block an SM and as many tiles in flight as fit.
+template <int DP, int NT>
+constexpr int kCtas = DP == 64 ? 3 : DP == 128 ? (NT == 1 ? 3 : 2) : 1;
 constexpr int round_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+constexpr int kSmallTiles = 8;  // of a block, at most, in the kernel for small calls
 
 struct Plan {
   PagedAttentionArgs a;
@@ -60,6 +75,8 @@ struct Plan {
   int head_tiles;  // items of a KV head
   int items;       // items of a sequence: hkv * head_tiles
   int tile;        // positions of a tile
+  int item_tiles;  // tiles of a sequence as long as the table
+  int cluster;     // blocks of an item (small calls); else 0
   int blocks;      // blocks of the attention kernel
   int max_len;     // positions the table has room for
   int join_warps;   // of a head in the joining kernel
@@ -125,6 +142,347 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// ---- A warp's work on a tile ---------------------------------------------------------------------
+
+// Per warp: K and V row of each position of the tile being loaded.
+using Rows = const void* [kWarpTile][2];
+
+// By a warp, lanes 0-15 a position each: looks up the rows of 16 positions of sequence b from `pos`
+// (this lane's) on, given this lane's page, writes the new token's row where it is among them, and
+// starts the copies of K and V to `dst`. Returns the mask of positions that count.
+template <class T, class S>
+__device__ __forceinline__ uint32_t load_tile(const Plan& p, Rows& rows, uint32_t dst, int b, int n,
+                                              int item, int pos, int page) {
+  const PagedAttentionArgs& a = p.a;
+  const PagedCache& c = a.cache;
+  const int lane = threadIdx.x % kWarp;
+  const int kv = item / p.head_tiles;
+  bool valid = false, append = false;
+  if (lane < kWarpTile) {
+    const void* k = c.k;
+    const void* v = c.v;
+    if (pos < n) {
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
+        const int off = pos - p.page.quotient(pos) * p.page.by;
+        valid = true;
+        append = a.k_new != nullptr && pos == n - 1;
+        k = static_cast<const T*>(c.k) + page * c.k_block + off * c.k_token + kv * c.k_head;
+        v = static_cast<const T*>(c.v) + page * c.v_block + off * c.v_token + kv * c.v_head;
+      } else {
+        atomicExch(p.status, kStatusBadPage);
+      }
+    }
+    *reinterpret_cast<ulonglong2*>(rows[lane]) =
+        make_ulonglong2(reinterpret_cast<uint64_t>(k), reinterpret_cast<uint64_t>(v));
+  }
+  const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+  const uint32_t fresh = __ballot_sync(0xffffffffu, append);
+  __syncwarp();
+  if (fresh) {
+    // the new token's row: to its slot (once for a KV head), and read from the call's tensors
+    const int64_t new_row = (static_cast<int64_t>(b) * c.hkv + kv) * c.dim;
+    const int row = __ffs(fresh) - 1;
+    if (item % p.head_tiles == 0) {
+      uint4* k = static_cast<uint4*>(const_cast<void*>(rows[row][0]));
+      uint4* v = static_cast<uint4*>(const_cast<void*>(rows[row][1]));
+      for (int i = lane; i < c.dim / 8; i += kWarp) {
+        k[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_new) + new_row)[i];
+        v[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v_new) + new_row)[i];
+      }
+    }
+    __syncwarp();
+    if (lane == row) {
+      rows[row][0] = static_cast<const T*>(a.k_new) + new_row;
+      rows[row][1] = static_cast<const T*>(a.v_new) + new_row;
+    }
+    __syncwarp();
+  }
+  // a lane copies the same chunk of every kStep-th row
+  constexpr int kStep = kWarp / S::kChunks;
+  const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
+  dst += row0 * S::kPitch + chunk * 16;
+  if (mask == 0xFFFFu && c.dim == S::kChunks * 8) {
+#pragma unroll
+    for (int i = 0; i < kWarpTile / kStep; ++i) {
+      const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(rows[row0 + i * kStep]);
+      const uint32_t to = dst + i * kStep * S::kPitch;
+      cp_async_16(to, reinterpret_cast<const char*>(kv_row.x) + chunk * 16);
+      cp_async_16(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + chunk * 16);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < kWarpTile / kStep; ++i) {
+      const int row = row0 + i * kStep;
+      const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(rows[row]);
+      const bool there = (mask >> row & 1) && chunk * 8 < c.dim;
+      const int at = there ? chunk * 16 : 0;
+      const uint32_t to = dst + i * kStep * S::kPitch;
+      cp_async_16_or_zero(to, reinterpret_cast<const char*>(kv_row.x) + at, there);
+      cp_async_16_or_zero(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + at, there);
+    }
+  }
+  __syncwarp();  // rows is rewritten by the next tile's
+  return mask;
+}
+
+// A warp's queries and sums for an item.
+template <class T, int DP, int NT, class S>
+struct Sums {
+  uint32_t qf[DP / 16][NT][2];
+  float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
+  float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the reference of all lanes (a maximum, at most kRise
+                             // below the largest score), this lane's sum
+
+  __device__ __forceinline__ void load_q(const Plan& p, int b, int item) {
+    const int dim = p.a.cache.dim, g = threadIdx.x % kWarp / 4, t2 = threadIdx.x % 4 * 2;
+    const int kv = item / p.head_tiles, h0 = item % p.head_tiles * S::kRows;
+    const T* q = static_cast<const T*>(p.a.q) +
+                 (static_cast<int64_t>(b) * p.a.hq + kv * p.group + h0) * dim;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = i * 8 + g, col = k * 16 + j * 8 + t2;
+          qf[k][i][j] = h0 + row < p.group && col < dim
+                            ? *reinterpret_cast<const uint32_t*>(q + row * dim + col)
+                            : 0u;
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      m[j][0] = m[j][1] = -INFINITY;
+      l[j][0] = l[j][1] = 0.0f;
+    }
+  }
+
+  // Adds the 16 positions at `tile`. scores: where this warp's go (kWeights). `after_qk` is called
+  // once the queries are not needed any more.
+  template <bool kWeights, class F>
+  __device__ __forceinline__ void add(const Plan& p, uint32_t tile, uint32_t mask, float* scores,
+                                      F after_qk) {
+    const int dim = p.a.cache.dim, lane = threadIdx.x % kWarp, g = lane / 4, t2 = lane % 4 * 2;
+    // the lanes' rows and chunks in the ldmatrix of K (positions 0-7, 8-15 by k 0-7, then by 8-15)
+    // and of V (positions 0-7 by dims 0-7, by 8-15, then positions 8-15)
+    const uint32_t k_at = tile + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kPitch + (lane >> 4) * 16;
+    const uint32_t v_at =
+        tile + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16 + S::kHalf;
+    // S^T: positions g, g + 8 by heads t2, t2 + 1
+    float s[NT][4] = {};
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      if (k * 16 < dim) {
+        uint32_t f[4];
+        ldmatrix_x4(f, k_at + k * 32);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma<T>(s[i], f, qf[k][i][0], qf[k][i][1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] *= p.a.scale_log2;
+    }
+    after_qk();
+    if (mask != 0xFFFFu) {
+      const bool at[2] = {(mask >> g & 1) != 0, (mask >> (g + 8) & 1) != 0};
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = at[j / 2] ? s[i][j] : -INFINITY;
+      }
+    }
+    if constexpr (kWeights) {
+      float* to = scores + g * p.score_rows;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if (i * 8 + t2 < p.score_rows) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            *reinterpret_cast<float2*>(to + r * 8 * p.score_rows + i * 8 + t2) =
+                make_float2(s[i][2 * r], s[i][2 * r + 1]);
+          }
+        }
+      }
+    }
+    float top[NT][2];
+    bool rises = false;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v = fmaxf(s[i][j], s[i][j + 2]);
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        top[i][j] = fmaxf(v, m[i][j]);
+        rises |= v > m[i][j] + kRise;
+      }
+    }
+    if (__any_sync(0xffffffffu, rises)) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f = m[i][j] == -INFINITY ? 0.0f : exp2_fast(m[i][j] - top[i][j]);
+          m[i][j] = top[i][j];
+          l[i][j] *= f;
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) {
+            o[d][i][j] *= f;
+            o[d][i][j + 2] *= f;
+          }
+        }
+      }
+    }
+    uint32_t hi[NT][2], lo[NT][2];  // positions t2, t2 + 1 (and + 8) by head g
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const float ref0 = m[i][0] == -INFINITY ? 0.0f : m[i][0];
+      const float ref1 = m[i][1] == -INFINITY ? 0.0f : m[i][1];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float p0 = exp2_fast(s[i][2 * r] - ref0), p1 = exp2_fast(s[i][2 * r + 1] - ref1);
+        l[i][0] += p0;
+        l[i][1] += p1;
+        const uint32_t h = pack2<T>(p0, p1);
+        const float2 back = unpack2<T>(h);
+        hi[i][r] = transposed(h);
+        lo[i][r] = transposed(pack2<T>(p0 - back.x, p1 - back.y));
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      if (d * 16 < dim) {
+        uint32_t f[4];
+        ldmatrix_x4_trans(f, v_at + d * 32);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, hi[i][0], hi[i][1]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, lo[i][0], lo[i][1]);
+      }
+    }
+  }
+
+  // By the block: the warps' sums together, into joined and ml[0]. Ends with a barrier.
+  __device__ __forceinline__ void join(float (&joined)[S::kRows][DP], float2 (&ml)[S::kWarps][S::kRows]) {
+    const int warp = threadIdx.x / kWarp, g = threadIdx.x % kWarp / 4, t2 = threadIdx.x % 4 * 2;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 4);
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 8);
+        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 16);
+        if (g == 0) ml[warp][i * 8 + t2 + j] = make_float2(m[i][j], l[i][j]);
+      }
+    }
+    __syncthreads();
+    float all_m[NT][2], all_l[NT][2], f[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) top = fmaxf(top, ml[w][i * 8 + t2 + j].x);
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) {
+          const float2 v = ml[w][i * 8 + t2 + j];
+          sum += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - top);
+        }
+        all_m[i][j] = top;
+        all_l[i][j] = sum;
+        f[i][j] = m[i][j] == -INFINITY ? 1.0f : exp2_fast(m[i][j] - top);
+      }
+    }
+    // the warps add their sums to one place in rounds, each to another share of the dimensions, so
+    // the order at every place is fixed and no warp waits for its turn
+#pragma unroll 1
+    for (int round = 0; round < S::kWarps; ++round) {
+      const int share = (warp + round) % S::kWarps;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        if (d % S::kWarps == share) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float* to = &joined[i * 8 + t2 + (j & 1)][d * 16 + g + j / 2 * 8];
+              const float v = o[d][i][j] * f[i][j & 1];
+              *to = round == 0 ? v : *to + v;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (warp == 0 && g == 0) {  // read by all warps above, before the rounds' barriers
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ml[0][i * 8 + t2 + j] = make_float2(all_m[i][j], all_l[i][j]);
+      }
+    }
+    __syncthreads();
+  }
+};
+
+// By a block of kThreads: adds the weights of `positions` positions of KV head kv of sequence b (n
+// long), from tile `tile0` of the sequence on, whose scores begin at tile `scores_tile`, for one item
+// (block `ht` of the head's query heads) whose rows have the sums row_lse.
+template <int kThreads>
+__device__ __forceinline__ void add_weights(const Plan& p, int b, int kv, int ht, int rows,
+                                            int scores_tile, int tile0, int positions, int n,
+                                            const float* row_lse) {
+  constexpr int kAtOnce = 2;
+  const PagedAttentionArgs& a = p.a;
+  const PagedCache& c = a.cache;
+  for (int i0 = threadIdx.x; i0 < positions; i0 += kAtOnce * kThreads) {
+    float* to[kAtOnce];
+    float w[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = i0 + k * kThreads, pos = tile0 * p.tile + i;
+      to[k] = nullptr;
+      w[k] = 0.0f;
+      if (i >= positions) continue;
+      const int block = p.page.quotient(pos);
+      const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + block];
+      const float2* s = reinterpret_cast<const float2*>(
+          p.scores + (static_cast<int64_t>(scores_tile) * p.tile + i) * p.score_rows);
+#pragma unroll 4
+      for (int r = 0; r < rows; r += 2) {
+        const float2 v = s[r / 2];
+        w[k] += exp2_fast(v.x - row_lse[r]);
+        if (r + 1 < rows) w[k] += exp2_fast(v.y - row_lse[r + 1]);
+      }
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
+        to[k] = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
+                (pos - block * static_cast<int>(p.page.by));
+        // a new token's slot may hold what its page was used for before
+        if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] += *to[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (to[k]) *to[k] = w[k];
+    }
+  }
+}
+
+// ---- Any call: all tiles over all blocks ---------------------------------------------------------
+
 // A position in the order of all tiles: sequence, item of the sequence, tile of the item.
 struct Walker {
   int b, item, tile, tiles, n;
@@ -151,20 +509,20 @@ struct Walker {
 
 template <int DP, int NT>
 struct Smem {
-  using S = Shape<DP, NT>;
+  using S = Shape<DP, NT, false>;
   alignas(128) unsigned char ring[S::kWarps][S::kStages][2][S::kHalf];
-  const void* rows[S::kWarps][kWarpTile][2];  // K and V row of each position of the tile being loaded
-  uint32_t mask[S::kWarps][S::kStages];       // positions that count
+  Rows rows[S::kWarps];
+  uint32_t mask[S::kWarps][S::kStages];  // positions that count
   float joined[S::kRows][DP];
   float2 ml[S::kWarps][S::kRows];
   int scan[S::kWarps];
-  int start[2];  // sequence of the block's first tile, tiles before it
+  int start[3];  // sequence of the block's first tile, tiles before it, its length
 };
 
 template <class T, int DP, int NT, bool kWeights>
-__global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
+__global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
     paged_attention_kernel(const __grid_constant__ Plan p) {
-  using S = Shape<DP, NT>;
+  using S = Shape<DP, NT, false>;
   constexpr int kTile = S::kTile, kThreads = S::kThreads, kWarps = S::kWarps;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   Smem<DP, NT>& sh = *reinterpret_cast<Smem<DP, NT>*>(smem_raw);
@@ -176,7 +534,8 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
 
   // Tiles before each sequence: a scan over the batch, a thread a sequence, in rounds. `find` is
-  // called with each thread's sequence and the tiles before and in it; returns the tiles in all.
+  // called with each thread's sequence, the tiles before and in it, and its length; returns the
+  // tiles in all.
   auto scan = [&](auto find) {
     int before = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
@@ -199,15 +558,15 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
         if (w < warp) t += sh.scan[w];
         sum += sh.scan[w];
       }
-      if (b < a.batch) find(b, before + t - own, own);
+      if (b < a.batch) find(b, before + t - own, own, n);
       before += sum;
       __syncthreads();  // sh.scan is written again
     }
     return before;
   };
   // a batch that fits one round keeps the scan's result in registers
-  int my_b = -1, my_before = 0, my_own = 0;
-  const int total = scan([&](int b, int before, int own) {
+  int my_b = -1, my_before = 0, my_own = 0, my_n = 0;
+  const int total = scan([&](int b, int before, int own, int n) {
     if (blockIdx.x == 0) {
       if (b == 0) p.first_tile[0] = 0;
       p.first_tile[b + 1] = before + own;
@@ -215,114 +574,52 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
     my_b = b;
     my_before = before;
     my_own = own;
+    my_n = n;
   });
   const Split split(total, p.blocks);
   const int t0 = split.start(blockIdx.x), t1 = split.start(blockIdx.x + 1);
   if (t0 >= t1) return;
-  auto is_start = [&](int b, int before, int own) {
+  auto is_start = [&](int b, int before, int own, int n) {
     if (before <= t0 && t0 < before + own) {
       sh.start[0] = b;
       sh.start[1] = before;
+      sh.start[2] = n;
     }
   };
   if (a.batch <= kThreads) {
-    if (my_b >= 0) is_start(my_b, my_before, my_own);
+    if (my_b >= 0) is_start(my_b, my_before, my_own, my_n);
     __syncthreads();
   } else {
     scan(is_start);
   }
   Walker load;
   load.b = sh.start[0];
-  load.enter<kTile>(p);
+  load.n = sh.start[2];
+  load.tiles = (load.n + kTile - 1) / kTile;
   load.item = (t0 - sh.start[1]) / load.tiles;
   load.tile = (t0 - sh.start[1]) % load.tiles;
   Walker now = load;
 
-  // ---- loading
   const uint32_t ring = smem_addr(sh.ring[warp]);
-  int load_tile = t0, load_stage = 0;
+  int load_at = t0, load_stage = 0;
   // the page of this lane's position in the tile to load next, read a tile ahead
   auto position = [&] { return load.tile * kTile + warp * kWarpTile + lane; };
   auto read_page = [&] {
     const int pos = position();
-    return lane < kWarpTile && load_tile < t1 && pos < load.n
+    return lane < kWarpTile && load_at < t1 && pos < load.n
                ? a.table[static_cast<int64_t>(load.b) * a.max_blocks + p.page.quotient(pos)]
                : -1;
   };
   int page = read_page();
   auto load_next = [&] {
-    if (load_tile < t1) {
-      const int kv = load.item / p.head_tiles;
-      bool valid = false, append = false;
-      if (lane < kWarpTile) {
-        const int pos = position();
-        const void* k = c.k;
-        const void* v = c.v;
-        if (pos < load.n) {
-          if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-            const int off = pos - p.page.quotient(pos) * p.page.by;
-            valid = true;
-            append = a.k_new != nullptr && pos == load.n - 1;
-            k = static_cast<const T*>(c.k) + page * c.k_block + off * c.k_token + kv * c.k_head;
-            v = static_cast<const T*>(c.v) + page * c.v_block + off * c.v_token + kv * c.v_head;
-          } else {
-            atomicExch(p.status, kStatusBadPage);
-          }
-        }
-        *reinterpret_cast<ulonglong2*>(sh.rows[warp][lane]) =
-            make_ulonglong2(reinterpret_cast<uint64_t>(k), reinterpret_cast<uint64_t>(v));
-      }
-      const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-      const uint32_t fresh = __ballot_sync(0xffffffffu, append);
+    if (load_at < t1) {
+      const uint32_t mask =
+          load_tile<T, S>(p, sh.rows[warp], ring + load_stage * 2 * S::kHalf, load.b, load.n,
+                          load.item, position(), page);
       if (lane == 0) sh.mask[warp][load_stage] = mask;
-      __syncwarp();
-      if (fresh) {
-        // the new token's row: to its slot (once for a KV head), and read from the call's tensors
-        const int64_t new_row = (static_cast<int64_t>(load.b) * c.hkv + kv) * c.dim;
-        const int row = __ffs(fresh) - 1;
-        if (load.item % p.head_tiles == 0) {
-          uint4* k = static_cast<uint4*>(const_cast<void*>(sh.rows[warp][row][0]));
-          uint4* v = static_cast<uint4*>(const_cast<void*>(sh.rows[warp][row][1]));
-          for (int i = lane; i < c.dim / 8; i += kWarp) {
-            k[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.k_new) + new_row)[i];
-            v[i] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v_new) + new_row)[i];
-          }
-        }
-        __syncwarp();
-        if (lane == row) {
-          sh.rows[warp][row][0] = static_cast<const T*>(a.k_new) + new_row;
-          sh.rows[warp][row][1] = static_cast<const T*>(a.v_new) + new_row;
-        }
-        __syncwarp();
-      }
       load.next<kTile>(p);
-      ++load_tile;
+      ++load_at;
       page = read_page();
-      // a lane copies the same chunk of every kStep-th row
-      constexpr int kStep = kWarp / S::kChunks;
-      const int chunk = lane % S::kChunks, row0 = lane / S::kChunks;
-      const uint32_t dst = ring + load_stage * 2 * S::kHalf + row0 * S::kPitch + chunk * 16;
-      if (mask == 0xFFFFu && c.dim == DP) {
-#pragma unroll
-        for (int i = 0; i < kWarpTile / kStep; ++i) {
-          const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(sh.rows[warp][row0 + i * kStep]);
-          const uint32_t to = dst + i * kStep * S::kPitch;
-          cp_async_16(to, reinterpret_cast<const char*>(kv_row.x) + chunk * 16);
-          cp_async_16(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + chunk * 16);
-        }
-      } else {
-#pragma unroll 4
-        for (int i = 0; i < kWarpTile / kStep; ++i) {
-          const int row = row0 + i * kStep;
-          const ulonglong2 kv_row = *reinterpret_cast<const ulonglong2*>(sh.rows[warp][row]);
-          const bool there = (mask >> row & 1) && chunk * 8 < c.dim;
-          const int at = there ? chunk * 16 : 0;
-          const uint32_t to = dst + i * kStep * S::kPitch;
-          cp_async_16_or_zero(to, reinterpret_cast<const char*>(kv_row.x) + at, there);
-          cp_async_16_or_zero(to + S::kHalf, reinterpret_cast<const char*>(kv_row.y) + at, there);
-        }
-      }
-      __syncwarp();  // sh.rows is rewritten by the next load
     }
     cp_async_commit();
     load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
@@ -330,48 +627,9 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
 #pragma unroll
   for (int s = 0; s < S::kStages - 1; ++s) load_next();
 
-  // ---- computing
-  const int g = lane / 4, t2 = lane % 4 * 2;
-  uint32_t qf[DP / 16][NT][2];
-  float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
-  float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the maximum of all lanes, this lane's sum
-  auto load_q = [&](const Walker& at) {
-    const int kv = at.item / p.head_tiles, h0 = at.item % p.head_tiles * S::kRows;
-    const T* q = static_cast<const T*>(a.q) +
-                 (static_cast<int64_t>(at.b) * a.hq + kv * p.group + h0) * c.dim;
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = i * 8 + g, col = k * 16 + j * 8 + t2;
-          qf[k][i][j] = h0 + row < p.group && col < c.dim
-                            ? *reinterpret_cast<const uint32_t*>(q + row * c.dim + col)
-                            : 0u;
-        }
-      }
-    }
-  };
-  auto begin = [&] {
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      m[j][0] = m[j][1] = -INFINITY;
-      l[j][0] = l[j][1] = 0.0f;
-    }
-  };
-  load_q(now);
-  begin();
-  // the lanes' rows and chunks in the ldmatrix of K (positions 0-7, 8-15 by k 0-7, then by 8-15)
-  // and of V (positions 0-7 by dims 0-7, by 8-15, then positions 8-15)
-  const uint32_t k_lane = ((lane & 7) + (lane >> 3 & 1) * 8) * S::kPitch + (lane >> 4) * 16;
-  const uint32_t v_lane = ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16 + S::kHalf;
-
+  Sums<T, DP, NT, S> sums;
+  sums.load_q(p, now.b, now.item);
+  sums.reset();
   int stage = 0, segment = t0;  // first tile of the current segment
   for (int t = t0; t < t1; ++t) {
     cp_async_wait<S::kStages - 2>();
@@ -380,176 +638,31 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
     const uint32_t mask = sh.mask[warp][stage];
     load_next();
     const bool item_ends = now.tile + 1 == now.tiles;
+    const bool changes = item_ends && t + 1 < t1;
     Walker following = now;
-    if (item_ends && t + 1 < t1) following.template next<kTile>(p);
-
+    if (changes) following.template next<kTile>(p);
+    // the next item's queries are on their way while this one is finished
+    const auto next_q = [&] {
+      if (changes) sums.load_q(p, following.b, following.item);
+    };
     if (mask != 0 || kWeights) {
-      // S^T: positions g, g + 8 by heads t2, t2 + 1
-      float s[NT][4] = {};
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        if (k * 16 < c.dim) {
-          uint32_t f[4];
-          ldmatrix_x4(f, tile + k_lane + k * 32);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma<T>(s[i], f, qf[k][i][0], qf[k][i][1]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] *= a.scale_log2;
-      }
-      // the next item's queries are on their way while this one is finished
-      if (item_ends && t + 1 < t1) load_q(following);
-      if (mask != 0xFFFFu) {
-        const bool at[2] = {(mask >> g & 1) != 0, (mask >> (g + 8) & 1) != 0};
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = at[j / 2] ? s[i][j] : -INFINITY;
-        }
-      }
-      if constexpr (kWeights) {
-        float* to = p.scores + (static_cast<int64_t>(t) * kTile + warp * kWarpTile + g) * p.score_rows;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if (i * 8 + t2 < p.score_rows) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              *reinterpret_cast<float2*>(to + r * 8 * p.score_rows + i * 8 + t2) =
-                  make_float2(s[i][2 * r], s[i][2 * r + 1]);
-            }
-          }
-        }
-      }
-      float top[NT][2];
-      bool rises = false;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float v = fmaxf(s[i][j], s[i][j + 2]);
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          top[i][j] = fmaxf(v, m[i][j]);
-          rises |= v > m[i][j];
-        }
-      }
-      if (__any_sync(0xffffffffu, rises)) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float f = m[i][j] == -INFINITY ? 0.0f : exp2_fast(m[i][j] - top[i][j]);
-            m[i][j] = top[i][j];
-            l[i][j] *= f;
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-              o[d][i][j] *= f;
-              o[d][i][j + 2] *= f;
-            }
-          }
-        }
-      }
-      uint32_t hi[NT][2], lo[NT][2];  // positions t2, t2 + 1 (and + 8) by head g
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const float ref0 = m[i][0] == -INFINITY ? 0.0f : m[i][0];
-        const float ref1 = m[i][1] == -INFINITY ? 0.0f : m[i][1];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float p0 = exp2_fast(s[i][2 * r] - ref0), p1 = exp2_fast(s[i][2 * r + 1] - ref1);
-          l[i][0] += p0;
-          l[i][1] += p1;
-          const uint32_t h = pack2<T>(p0, p1);
-          const float2 back = unpack2<T>(h);
-          hi[i][r] = transposed(h);
-          lo[i][r] = transposed(pack2<T>(p0 - back.x, p1 - back.y));
-        }
-      }
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        if (d * 16 < c.dim) {
-          uint32_t f[4];
-          ldmatrix_x4_trans(f, tile + v_lane + d * 32);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, hi[i][0], hi[i][1]);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma<T>(o[d][i], f, lo[i][0], lo[i][1]);
-        }
-      }
+      sums.template add<kWeights>(
+          p, tile, mask,
+          kWeights ? p.scores + (static_cast<int64_t>(t) * kTile + warp * kWarpTile) * p.score_rows
+                   : nullptr,
+          next_q);
+    } else {
+      next_q();
     }
-    if (mask == 0 && !kWeights && item_ends && t + 1 < t1) load_q(following);
     __syncwarp();  // this stage is refilled by the next load_next
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
-
-    // ---- the end of a segment: join the warps
     if (!item_ends && t + 1 < t1) {
       ++now.tile;
       continue;
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 4);
-        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 8);
-        l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 16);
-        if (g == 0) sh.ml[warp][i * 8 + t2 + j] = make_float2(m[i][j], l[i][j]);
-      }
-    }
-    __syncthreads();
-    float all_m[NT][2], all_l[NT][2], f[NT][2];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.ml[w][i * 8 + t2 + j].x);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 v = sh.ml[w][i * 8 + t2 + j];
-          sum += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - top);
-        }
-        all_m[i][j] = top;
-        all_l[i][j] = sum;
-        f[i][j] = m[i][j] == -INFINITY ? 1.0f : exp2_fast(m[i][j] - top);
-      }
-    }
-    // the warps add their sums to one place in rounds, each to another share of the dimensions, so
-    // the order at every place is fixed and no warp waits for its turn
-#pragma unroll 1
-    for (int round = 0; round < kWarps; ++round) {
-      const int share = (warp + round) % kWarps;
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        if (d % kWarps == share) {
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float* to = &sh.joined[i * 8 + t2 + (j & 1)][d * 16 + g + j / 2 * 8];
-              const float v = o[d][i][j] * f[i][j & 1];
-              *to = round == 0 ? v : *to + v;
-            }
-          }
-        }
-      }
-      __syncthreads();
-    }
-    if (warp == 0 && g == 0) {  // read by all warps above, before the loop's barriers
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sh.ml[0][i * 8 + t2 + j] = make_float2(all_m[i][j], all_l[i][j]);
-        }
-      }
-    }
-    __syncthreads();
+
+    // the end of a segment
+    sums.join(sh.joined, sh.ml);
     const int kv = now.item / p.head_tiles, h0 = now.item % p.head_tiles * S::kRows;
     const int rows = min(p.group - h0, S::kRows);
     const int head = kv * p.group + h0;
@@ -574,12 +687,168 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
       if (tid < rows) p.part_ml[slot * S::kRows + tid] = sh.ml[0][tid];
     }
     __syncthreads();  // joined and ml are written again by the next segment
-    if (t + 1 < t1) {
+    if (changes) {
       now = following;
       segment = t + 1;
-      begin();
+      sums.reset();
     }
   }
+}
+
+// ---- Small calls: a cluster of blocks an item ----------------------------------------------------
+//
+// Block r of an item's R takes its tiles r, r + R, ...: which tiles a block has does not depend on
+// the length, so the pages of all of them are looked up while the length is on its way.
+template <int DP, int NT>
+struct SmallSmem {
+  using S = Shape<DP, NT, true>;
+  alignas(128) unsigned char ring[S::kWarps][S::kStages][2][S::kHalf];
+  Rows rows[S::kWarps];
+  int pages[S::kWarps][kSmallTiles][kWarpTile];
+  uint32_t mask[S::kWarps][S::kStages];
+  float joined[S::kRows][DP];
+  float2 ml[S::kWarps][S::kRows];
+  float share[S::kRows][kMaxCluster];  // of the blocks of the cluster in a row's result
+  float row_lse[S::kRows];
+};
+
+template <class T, int DP, int NT, bool kWeights>
+__global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
+    paged_attention_small_kernel(const __grid_constant__ Plan p) {
+  using S = Shape<DP, NT, true>;
+  constexpr int kTile = S::kTile, kThreads = S::kThreads;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  SmallSmem<DP, NT>& sh = *reinterpret_cast<SmallSmem<DP, NT>*>(smem_raw);
+  wait_then_release();
+  const PagedAttentionArgs& a = p.a;
+  const PagedCache& c = a.cache;
+  const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
+  const int ranks = p.cluster, rank = blockIdx.x % ranks, index = blockIdx.x / ranks;
+  const int b = index / p.items, item = index % p.items;
+
+  // the pages of this warp's positions, two of the block's tiles at a time
+  const int own_most = (p.item_tiles - rank + ranks - 1) / ranks;  // tiles of the longest sequence
+#pragma unroll
+  for (int k = 0; k < kSmallTiles / 2; ++k) {
+    const int i = 2 * k + lane / kWarpTile;
+    const int pos = (rank + i * ranks) * kTile + warp * kWarpTile + lane % kWarpTile;
+    if (i < own_most) {
+      sh.pages[warp][i][lane % kWarpTile] =
+          pos < p.max_len ? a.table[static_cast<int64_t>(b) * a.max_blocks + p.page.quotient(pos)] : -1;
+    }
+  }
+  const int given = a.lens[b];
+  Sums<T, DP, NT, S> sums;
+  sums.load_q(p, b, item);
+  sums.reset();
+  const int n = clamped(p, given);
+  if (given != n && tid == 0) atomicExch(p.status, kStatusBadPage);
+  const int tiles = (n + kTile - 1) / kTile;
+  const int own = tiles > rank ? (tiles - rank + ranks - 1) / ranks : 0;
+
+  const uint32_t ring = smem_addr(sh.ring[warp]);
+  __syncwarp();
+  int loaded = 0, load_stage = 0, stage = 0;
+  auto load_next = [&] {
+    if (loaded < own) {
+      const uint32_t mask = load_tile<T, S>(
+          p, sh.rows[warp], ring + load_stage * 2 * S::kHalf, b, n, item,
+          (rank + loaded * ranks) * kTile + warp * kWarpTile + lane,
+          sh.pages[warp][loaded][lane % kWarpTile]);
+      if (lane == 0) sh.mask[warp][load_stage] = mask;
+      ++loaded;
+    }
+    cp_async_commit();
+    load_stage = load_stage + 1 == S::kStages ? 0 : load_stage + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < S::kStages - 1; ++i) load_next();
+#pragma unroll 1
+  for (int i = 0; i < own; ++i) {
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();
+    const uint32_t tile = ring + stage * 2 * S::kHalf;
+    const uint32_t mask = sh.mask[warp][stage];
+    load_next();
+    if (mask != 0 || kWeights) {
+      const int64_t t = static_cast<int64_t>(index) * p.item_tiles + rank + i * ranks;
+      sums.template add<kWeights>(
+          p, tile, mask,
+          kWeights ? p.scores + (t * kTile + warp * kWarpTile) * p.score_rows : nullptr, [] {});
+    }
+    __syncwarp();  // this stage is refilled by the next load_next
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+  }
+
+  const int kv = item / p.head_tiles, h0 = item % p.head_tiles * S::kRows;
+  const int rows = min(p.group - h0, S::kRows);
+  T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(b) * a.hq + kv * p.group + h0) * c.dim;
+  if (tiles == 0) {  // so for every block of the cluster
+    for (int i = rank * kThreads + tid; i < rows * c.dim; i += ranks * kThreads) {
+      out[i] = from_f32<T>(0.0f);
+    }
+    return;
+  }
+  // every block takes a share of the output and the weights of its own tiles; one without tiles has
+  // sums of 0 and a maximum of -inf
+  sums.join(sh.joined, sh.ml);
+  const cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int pairs = c.dim / 2;
+  const int first = rank * kThreads + tid;
+  float2 v[kMaxCluster];
+  auto read = [&](int i) {
+    const int row = i / pairs, d = i % pairs * 2;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      v[r] = r < ranks && i < rows * pairs
+                 ? *reinterpret_cast<const float2*>(&cluster.map_shared_rank(&sh, r)->joined[row][d])
+                 : make_float2(0.0f, 0.0f);
+    }
+  };
+  read(first);
+  if (tid < rows) {
+    float2 ml[kMaxCluster];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      ml[r] = r < ranks ? cluster.map_shared_rank(&sh, r)->ml[0][tid] : make_float2(-INFINITY, 0.0f);
+      m = fmaxf(m, ml[r].x);
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      // a part whose scores are all -inf is not scaled: its sums are 0, or NaN
+      ml[r].x = ml[r].x == -INFINITY ? 1.0f : exp2_fast(ml[r].x - m);
+      l = fmaf(ml[r].y, ml[r].x, l);
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) sh.share[tid][r] = ml[r].x / l;
+    sh.row_lse[tid] = m + log2f(l);
+  }
+  __syncthreads();
+  for (int i = first; i < rows * pairs; i += ranks * kThreads) {
+    if (i != first) read(i);
+    const int row = i / pairs, d = i % pairs * 2;
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      if (r < ranks) {
+        sum.x = fmaf(v[r].x, sh.share[row][r], sum.x);
+        sum.y = fmaf(v[r].y, sh.share[row][r], sum.y);
+      }
+    }
+    *reinterpret_cast<uint32_t*>(out + row * c.dim + d) = pack2<T>(sum.x, sum.y);
+  }
+  // the others read this block's part up to here; the barrier's second half is at the end
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if constexpr (kWeights) {
+    for (int i = 0; i < own; ++i) {
+      const int tile = rank + i * ranks;
+      add_weights<kThreads>(p, b, kv, 0, rows, index * p.item_tiles + tile, tile,
+                            min(kTile, n - tile * kTile), n, sh.row_lse);
+    }
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- Joining -------------------------------------------------------------------------------------
@@ -591,7 +860,6 @@ __global__ void __launch_bounds__(Shape<DP, NT>::kThreads, Shape<DP, NT>::kCtas)
 // positions at a time.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / kWarp;
-constexpr int kMaxDim = 256;
 
 // Reads of the attention kernel's workspace
 struct Parts {
@@ -712,11 +980,10 @@ __device__ __forceinline__ void join_head(const Plan& p) {
   }
 }
 
-__device__ __forceinline__ void add_weights(const Plan& p, int block, int blocks) {
+__device__ __forceinline__ void join_weights(const Plan& p, int block, int blocks) {
   __shared__ float row_lse[16];
   __shared__ int start;
   const PagedAttentionArgs& a = p.a;
-  const PagedCache& c = a.cache;
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
   // tiles of (sequence, KV head), the items of a KV head together
   const int total = p.first_tile[a.batch];
@@ -750,39 +1017,8 @@ __device__ __forceinline__ void add_weights(const Plan& p, int block, int blocks
         }
       }
       __syncthreads();
-      constexpr int kAtOnce = 2;
-      const int positions = min(count * p.tile, n - tile0 * p.tile);
-      for (int i0 = tid; i0 < positions; i0 += kAtOnce * kJoinThreads) {
-        float* to[kAtOnce];
-        float w[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-          const int i = i0 + k * kJoinThreads, pos = tile0 * p.tile + i;
-          to[k] = nullptr;
-          w[k] = 0.0f;
-          if (i >= positions) continue;
-          const int block = p.page.quotient(pos);
-          const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + block];
-          const float2* s = reinterpret_cast<const float2*>(
-              p.scores + (static_cast<int64_t>(begin + tile0) * p.tile + i) * p.score_rows);
-#pragma unroll 4
-          for (int r = 0; r < rows; r += 2) {
-            const float2 v = s[r / 2];
-            w[k] += exp2_fast(v.x - row_lse[r]);
-            if (r + 1 < rows) w[k] += exp2_fast(v.y - row_lse[r + 1]);
-          }
-          if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-            to[k] = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
-                    (pos - block * static_cast<int>(p.page.by));
-            // a new token's slot may hold what its page was used for before
-            if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] += *to[k];
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) {
-          if (to[k]) *to[k] = w[k];
-        }
-      }
+      add_weights<kJoinThreads>(p, b, kv, ht, rows, begin + tile0, tile0,
+                                min(count * p.tile, n - tile0 * p.tile), n, row_lse);
       __syncthreads();  // row_lse is rewritten
     }
     t += count;
@@ -795,7 +1031,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (static_cast<int>(blockIdx.x) < p.join_blocks) {
     join_head<T>(p);
   } else if constexpr (kWeights) {
-    add_weights(p, blockIdx.x - p.join_blocks, gridDim.x - p.join_blocks);
+    join_weights(p, blockIdx.x - p.join_blocks, gridDim.x - p.join_blocks);
   }
 }
 
@@ -814,26 +1050,45 @@ auto with_shape(int dim, int group, F f) {
 
 int64_t aligned_up(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Fills the plan's sizes and, with a workspace, its pointers; returns the workspace's bytes.
+// Fills the plan's sizes and, with a workspace, its pointers; returns the workspace's bytes, or -1
+// where the sizes are out of range.
 int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
   p->a = a;
   p->group = a.hq / a.cache.hkv;
-  int ctas = 1;
+  int ctas = 1, small_tile = 1;
   with_shape(a.cache.dim, p->group, [&]<int DP, int NT>() {
-    p->rows = Shape<DP, NT>::kRows;
-    p->tile = Shape<DP, NT>::kTile;
-    ctas = Shape<DP, NT>::kCtas;
+    p->rows = Shape<DP, NT, false>::kRows;
+    p->tile = Shape<DP, NT, false>::kTile;
+    ctas = kCtas<DP, NT>;
+    small_tile = Shape<DP, NT, true>::kTile;
   });
   p->head_tiles = (p->group + p->rows - 1) / p->rows;
   const int64_t items = static_cast<int64_t>(a.cache.hkv) * p->head_tiles;
   const int64_t len = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
-  const int64_t tiles = a.batch * items * ((len + p->tile - 1) / p->tile);
+  // A small call: clusters as large as there is room for at one block an SM and as every block has a
+  // tile, if that leaves no block more than kSmallTiles. The weights of a KV head need all its query
+  // heads in one item.
+  const int64_t all_items = a.batch * items, small_tiles = (len + small_tile - 1) / small_tile;
+  p->cluster = 0;
+  if (all_items > 0 && all_items <= sm_count() && small_tiles > 0 &&
+      (!a.cache.weights || p->head_tiles == 1)) {
+    int cluster = 1;
+    while (cluster < kMaxCluster && all_items * cluster * 2 <= sm_count() && cluster < small_tiles) {
+      cluster *= 2;
+    }
+    if (small_tiles <= static_cast<int64_t>(kSmallTiles) * cluster) {
+      p->cluster = cluster;
+      p->tile = small_tile;
+    }
+  }
+  const int64_t tiles = all_items * ((len + p->tile - 1) / p->tile);
   if (len > INT32_MAX - p->tile || tiles > INT32_MAX / 2 ||
       static_cast<int64_t>(a.batch) * a.hq > INT32_MAX / 4) {
-    return 0;
+    return -1;
   }
   p->items = static_cast<int>(items);
   p->max_len = static_cast<int>(len);
+  p->item_tiles = static_cast<int>((len + p->tile - 1) / p->tile);
   p->score_rows = (std::min(p->group, p->rows) + 1) / 2 * 2;
   p->page = Divider(static_cast<uint32_t>(a.cache.block_size));
   const int64_t resident = static_cast<int64_t>(sm_count()) * ctas;
@@ -849,11 +1104,15 @@ int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
     at += aligned_up(bytes);
     return static_cast<unsigned char*>(a.workspace) + here;
   };
-  p->part_o = reinterpret_cast<float*>(take(2LL * p->blocks * p->rows * a.cache.dim * 4));
-  p->part_ml = reinterpret_cast<float2*>(take(2LL * p->blocks * p->rows * 8));
-  p->first_tile = reinterpret_cast<int*>(take((a.batch + 1LL) * 4));
+  if (!p->cluster) {
+    p->part_o = reinterpret_cast<float*>(take(2LL * p->blocks * p->rows * a.cache.dim * 4));
+    p->part_ml = reinterpret_cast<float2*>(take(2LL * p->blocks * p->rows * 8));
+    p->first_tile = reinterpret_cast<int*>(take((a.batch + 1LL) * 4));
+    if (a.cache.weights) {
+      p->lse = reinterpret_cast<float*>(take(static_cast<int64_t>(a.batch) * a.hq * 4));
+    }
+  }
   if (a.cache.weights) {
-    p->lse = reinterpret_cast<float*>(take(static_cast<int64_t>(a.batch) * a.hq * 4));
     p->scores = reinterpret_cast<float*>(take(tiles * p->tile * p->score_rows * 4));
   }
   return at;
@@ -868,10 +1127,20 @@ cudaError_t launch(const Plan& p, cudaStream_t stream) {
   std::call_once(once[dev & 63], [&] {
     err = cudaFuncSetAttribute(paged_attention_kernel<T, DP, NT, kWeights>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Smem<DP, NT>));
+    if (err != cudaSuccess) return;
+    err = cudaFuncSetAttribute(paged_attention_small_kernel<T, DP, NT, kWeights>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               sizeof(SmallSmem<DP, NT>));
   });
   if (err != cudaSuccess) return err;
+  if (p.cluster) {
+    return launch_serialised(paged_attention_small_kernel<T, DP, NT, kWeights>,
+                             dim3(p.a.batch * p.items * p.cluster),
+                             dim3(Shape<DP, NT, true>::kThreads), sizeof(SmallSmem<DP, NT>), stream,
+                             p.cluster, p);
+  }
   err = launch_serialised(paged_attention_kernel<T, DP, NT, kWeights>, dim3(p.blocks),
-                          dim3(Shape<DP, NT>::kThreads), sizeof(Smem<DP, NT>), stream, 1, p);
+                          dim3(Shape<DP, NT, false>::kThreads), sizeof(Smem<DP, NT>), stream, 1, p);
   if (err != cudaSuccess) return err;
   return launch_serialised(paged_join_kernel<T, kWeights>,
                            dim3(p.join_blocks + (kWeights ? 8 * sm_count() : 0)),

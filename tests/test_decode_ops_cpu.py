@@ -91,7 +91,7 @@ def test_attention_argument_errors():
     assert attend(c, q=FAKE + 4) == ("paged_attention: q, out, k_new and v_new must be 16-byte aligned")
     size = capi.lib().int4gemv_paged_attention_workspace_size
     need = size(ctypes.addressof(c), 3, 4, 5, 1)
-    assert need > size(ctypes.addressof(c), 3, 4, 5, 0) > 0
+    assert need > size(ctypes.addressof(c), 3, 4, 5, 0) >= 0
     for ws, have in ((None, need), (FAKE, need - 1), (FAKE + 16, need)):
         with pytest.raises(capi.CapiError, match=f"workspace of {need} bytes") as e:
             capi.call("int4gemv_paged_attention", FAKE, FAKE, ctypes.addressof(c), FAKE, FAKE, 1.0,
