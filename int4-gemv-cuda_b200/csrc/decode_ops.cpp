@@ -1,6 +1,7 @@
 // The torch binding of the decode-step operators (add_rms_norm, paged_attention, paged_evict,
 // token_logprobs): tensor checks, outputs and workspace from torch's caching allocator, and the
 // call of the C ABI on torch's current stream. Nothing synchronises.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -15,6 +16,12 @@ void check_status(int status) { TORCH_CHECK(status == INT4GEMV_OK, int4gemv_last
 
 void* stream_of(const at::Tensor& t) {
   return static_cast<void*>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
+}
+
+// An uninitialised contiguous tensor on the device of `like`, from the caching allocator without
+// torch's operator dispatch (a small call's time on the host is mostly such calls: 0.5 us less each).
+at::Tensor make(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
 }
 
 int dtype_of(const char* name, const char* what, const at::Tensor& t, bool f32) {
@@ -56,7 +63,7 @@ Norm check_norm(const char* name, const at::Tensor& x, const at::Tensor& weight,
   check_like(name, "weight", weight, x.scalar_type(), {x.size(1)}, x);
   if (!residual.has_value()) return {dtype, x, nullptr, nullptr};
   check_like(name, "residual", *residual, x.scalar_type(), x.sizes(), x);
-  at::Tensor h = at::empty(x.sizes(), x.options());
+  at::Tensor h = make(x.sizes(), x.scalar_type(), x);
   return {dtype, h, residual->data_ptr(), h.data_ptr()};
 }
 
@@ -105,7 +112,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const at::T
   const char* name = "add_rms_norm";
   const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::make_optional(x.device()) : c10::nullopt);
   const Norm n = check_norm(name, x, weight, residual);
-  at::Tensor y = at::empty(x.sizes(), x.options());
+  at::Tensor y = make(x.sizes(), x.scalar_type(), x);
   check_status(int4gemv_add_rms_norm(y.data_ptr(), n.h_out, x.data_ptr(), n.residual,
                                      weight.data_ptr(), static_cast<float>(eps), n.dtype, x.size(0),
                                      x.size(1), stream_of(x)));
@@ -118,8 +125,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant(
   const char* name = "add_rms_norm_quant";
   const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::make_optional(x.device()) : c10::nullopt);
   const Norm n = check_norm(name, x, weight, residual);
-  at::Tensor y = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor scales = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  at::Tensor y = make(x.sizes(), at::kFloat8_e4m3fn, x);
+  at::Tensor scales = make({x.size(0)}, at::kFloat, x);
   check_status(int4gemv_add_rms_norm_quant(y.data_ptr(), scales.data_ptr<float>(), n.h_out,
                                            x.data_ptr(), n.residual, weight.data_ptr(),
                                            static_cast<float>(eps), n.dtype, x.size(0), x.size(1),
@@ -152,9 +159,9 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   const int64_t blocks = block_table.size(1);
   const int64_t bytes = int4gemv_paged_attention_workspace_size(&cache, batch, q_heads, blocks, w != nullptr);
   TORCH_CHECK(bytes >= 0, int4gemv_last_error());
-  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor out = make(q.sizes(), q.scalar_type(), q);
   at::Tensor workspace;
-  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (bytes > 0) workspace = make({bytes}, at::kByte, q);
   check_status(int4gemv_paged_attention(
       out.data_ptr(), q.data_ptr(), &cache, block_table.data_ptr<int>(), seq_lens.data_ptr<int>(),
       static_cast<float>(scale), k.has_value() ? k->data_ptr() : nullptr,
@@ -177,8 +184,8 @@ std::tuple<at::Tensor, at::Tensor> paged_evict(const at::Tensor& k_cache, const 
   check_table(name, "new_table", new_table, batch, k_cache);
   TORCH_CHECK(budget > 0, name, ": budget ", budget, " must be positive");
   const c10::cuda::CUDAGuard guard(k_cache.device());
-  at::Tensor kept = at::empty({batch, cache.kv_heads, budget}, seq_lens.options());
-  at::Tensor new_lens = at::empty({batch}, seq_lens.options());
+  at::Tensor kept = make({batch, cache.kv_heads, budget}, at::kInt, k_cache);
+  at::Tensor new_lens = make({batch}, at::kInt, k_cache);
   check_status(int4gemv_paged_evict(kept.data_ptr<int>(), new_lens.data_ptr<int>(), &cache,
                                     block_table.data_ptr<int>(), seq_lens.data_ptr<int>(),
                                     new_table.data_ptr<int>(), budget, recent, batch,
@@ -200,10 +207,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_logprobs(const 
   TORCH_CHECK(top >= 0 && top <= INT4GEMV_MAX_TOP && top <= vocab, name, ": top ", top,
               " must be in [0, ", INT4GEMV_MAX_TOP, "] and at most vocab = ", vocab);
   const c10::cuda::CUDAGuard guard(logits.device());
-  const auto f32 = logits.options().dtype(at::kFloat);
-  at::Tensor logprobs = at::empty({rows}, f32), entropy = at::empty({rows}, f32);
-  at::Tensor top_logprobs = at::empty({rows, top}, f32);
-  at::Tensor top_ids = at::empty({rows, top}, tokens.options());
+  at::Tensor logprobs = make({rows}, at::kFloat, logits), entropy = make({rows}, at::kFloat, logits);
+  at::Tensor top_logprobs = make({rows, top}, at::kFloat, logits);
+  at::Tensor top_ids = make({rows, top}, at::kLong, logits);
   check_status(int4gemv_token_logprobs(
       logprobs.data_ptr<float>(), entropy.data_ptr<float>(), top_logprobs.data_ptr<float>(),
       top_ids.data_ptr<int64_t>(), logits.data_ptr(), tokens.data_ptr<int64_t>(), dtype, rows, vocab,
