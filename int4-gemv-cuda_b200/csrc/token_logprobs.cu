@@ -51,7 +51,7 @@ constexpr int kGroups = 64;    // groups of threads whose maxima give the thresh
 constexpr int kList = 512;     // places of the list: tiles of threads
 constexpr int kPicks = 128;    // of them, those that reach the last threshold
 constexpr int kKeys = 512;     // elements that are ranked
-constexpr int kAtOnce = 4;     // picks a warp reads at once
+constexpr int kAtOnce = 2;     // picks a warp reads at once
 constexpr int kMaxCluster = 8;
 constexpr float kFar = 65536.0f;  // the largest maximum whose sums the one pass holds
 constexpr float kLn2 = 0.69314718055994531f;
@@ -454,12 +454,13 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
 
     int tile = 0;
     float least = -INFINITY;
-    int renew_at = 0;
+    int renew_at = 0, last_slot = 0;
     for (int base = r.c0; base < r.c1; base += kTile, ++tile) {
       cp_async_wait<kRing - 2>();
       uint4 now[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; ++j) now[j] = ld_shared_v4(in + j * kThreads * 16);
+      last_slot = (in - ring) / kSlot;
       in = in + kSlot == ring_end ? ring : in + kSlot;
       fetch();
       uint32_t most = max_words<T>(now[0]);
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
       sums.u = u.x + u.y;
     }
     if constexpr (kTop) {
-      if (r.c0 < r.c1) publish(sh, sums.m);
+      if (tile > 1) publish(sh, sums.m);
     }
 
     // the block's sums
@@ -519,7 +520,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
     __syncthreads();
     uint32_t least_key = 0;
     if constexpr (kTop) {
-      least_key = block_threshold(sh, a.top);
+      // the maxima of a row of one tile are those of its first threshold
+      least_key = tile == 1 ? sh.threshold : block_threshold(sh, a.top);
       if (sh.listed > kList) remake_list<T>(sh, r, a.vocab, least_key);
       // the elements of the entries that reach the threshold, a lane an element
       const int listed = min(sh.listed, kList);
@@ -541,7 +543,14 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
           const int c = r.c0 + (e < picked ? sh.picks[e] : 0) + lane / E * kThreads;
           index[i] = c * E - r.shift + lane % E;
           if (e >= picked || lane >= kPer * E || c >= r.c1 || index[i] >= a.vocab) index[i] = -1;
-          x[i] = index[i] >= 0 ? to_f32(r.row[index[i]]) : 0.0f;
+          // the last tile is still in its slots
+          x[i] = 0.0f;
+          if (index[i] >= 0) {
+            const int in_tile = sh.picks[e] - (tile - 1) * kTile;
+            x[i] = to_f32(in_tile >= 0 ? reinterpret_cast<const T*>(
+                                             &sh.ring[last_slot][lane / E][in_tile])[lane % E]
+                                       : r.row[index[i]]);
+          }
         }
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
@@ -620,12 +629,20 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
       for (int q = 0; q < ranks; ++q) total += sh.parts[q].count;
       if (p < ranks && i < sh.parts[p].count) {
         const Key mine = sh.parts[p].top[i];
-        int better = i;  // a part's own entries are in order
-        for (int q = 0; q < ranks; ++q) {
-          if (q == p) continue;
-          const int count = sh.parts[q].count;
-#pragma unroll 8
-          for (int j = 0; j < count; ++j) better += sh.parts[q].top[j] > mine;
+        // a part's entries are in order: its own come before it, of the others a binary search
+        // counts those that are larger
+        int better = i;
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) {
+          if (q >= ranks || q == p) continue;
+          const Part& other = sh.parts[q];
+          int larger = 0;
+#pragma unroll
+          for (int step = kMaxTop / 2; step > 0; step /= 2) {
+            if (larger + step <= other.count && other.top[larger + step - 1] > mine) larger += step;
+          }
+          if (larger < other.count && other.top[larger] > mine) ++larger;
+          better += larger;
         }
         if (better < a.top) {
           top_logprobs[better] = logprob(key_value(mine));
