@@ -5,10 +5,12 @@
 // its squares and the store. The 8-bit output needs max|y| = max|h w| / rms, so the same reduction
 // carries max|h w| beside the sum and the row still needs no second one.
 //
-// Layout: rows of whole 16-byte chunks go to blocks that stay for many rows: a thread holds its
-// chunks of the weight throughout and fetches the next row while this one is summed and stored.
-// Other rows (odd lengths, unaligned tensors) are cut into the chunks of memory they lie in, so that
-// they still move whole chunks and only their first and last one by elements.
+// Layout: a row is cut into the 16-byte chunks of memory it lies in, so that a row of odd length
+// (whose start falls inside a chunk) still moves whole chunks; only the stores of its first and last
+// one go by elements. Blocks stay for many rows: a thread holds its chunks of the weight throughout
+// and fetches the next row while this one is summed and stored. A block's rows are a multiple of a
+// chunk's elements apart, so they all start at the same place of a chunk. Unaligned tensors and rows
+// of more than 2048 chunks take a plain loop that reads the row twice.
 //
 // Bound by HBM: x, residual, h and y move once each.
 #include <algorithm>
@@ -20,7 +22,10 @@ namespace i4 {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
-constexpr int kRowThreads = 1024;  // threads an SM gets for rows of whole chunks
+constexpr int kRowThreads = 1024;  // threads an SM gets
+// Threads of a block whose threads take kPer chunks: 544 of two leave room for a second block where
+// rows of 8192 elements and a bit have 1025 chunks.
+constexpr int most_threads(bool whole, int per) { return whole || per == 1 ? 1024 : per == 2 ? 544 : 704; }
 constexpr float kScaleFloor = 1e-12f;  // a row of zeros still has a scale to divide by
 
 // Four / eight e4m3 values of y, saturating (a NaN stays one).
@@ -85,33 +90,65 @@ struct NormRow {
       each<T>(c, [&](int i, int e) { w.v[i] = to_f32(p[e]); });
     }
   }
+  // Elements [lo, hi) of chunk c are inside of the row.
   template <class T>
+  __device__ __forceinline__ void inside(int c, int& lo, int& hi) const {
+    constexpr int E = Chunk<T>::kElems;
+    lo = max(shift - c * E, 0);
+    hi = min(shift + a.hidden - c * E, E);
+  }
+  template <class T, bool kWhole = false>
   __device__ __forceinline__ void store(int c, void* to, const Chunk<T>& v) const {
     constexpr int E = Chunk<T>::kElems;
-    T* p = static_cast<T*>(to) + row0;
-    if (whole<T>(c)) {
-      *reinterpret_cast<uint4*>(p + (c * E - shift)) = v.get();
+    T* p = static_cast<T*>(to) + row0 + (c * E - shift);
+    if (kWhole || whole<T>(c)) {
+      *reinterpret_cast<uint4*>(p) = v.get();
+    } else if (a.aligned) {  // by 32-bit words, and halves of those at the ends
+      int lo, hi;
+      inside<T>(c, lo, hi);
+      const uint4 u = v.get();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t word = word_of4(u, j);
+        if constexpr (sizeof(T) == 4) {
+          if (j >= lo && j < hi) reinterpret_cast<uint32_t*>(p)[j] = word;
+        } else {
+          const bool first = 2 * j >= lo && 2 * j < hi, second = 2 * j + 1 >= lo && 2 * j + 1 < hi;
+          if (first && second) {
+            reinterpret_cast<uint32_t*>(p)[j] = word;
+          } else if (first) {
+            reinterpret_cast<uint16_t*>(p)[2 * j] = static_cast<uint16_t>(word);
+          } else if (second) {
+            reinterpret_cast<uint16_t*>(p)[2 * j + 1] = static_cast<uint16_t>(word >> 16);
+          }
+        }
+      }
     } else {
-      each<T>(c, [&](int i, int e) { p[e] = from_f32<T>(v.v[i]); });
+      each<T>(c, [&](int i, int) { p[i] = from_f32<T>(v.v[i]); });
     }
   }
-  template <class T>
+  template <class T, bool kWhole = false>
   __device__ __forceinline__ void store_e4m3(int c, const Chunk<T>& v) const {
     constexpr int E = Chunk<T>::kElems;
-    uint8_t* p = static_cast<uint8_t*>(a.y) + row0;
+    uint8_t* p = static_cast<uint8_t*>(a.y) + row0 + (c * E - shift);
     uint32_t w[E / 4];
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
       w[i] = e4m3x4(v.v[4 * i], v.v[4 * i + 1], v.v[4 * i + 2], v.v[4 * i + 3]);
     }
-    if (whole<T>(c)) {
+    if (kWhole || whole<T>(c)) {
       if constexpr (E == 8) {
-        *reinterpret_cast<uint2*>(p + (c * E - shift)) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
       } else {
-        *reinterpret_cast<uint32_t*>(p + (c * E - shift)) = w[0];
+        *reinterpret_cast<uint32_t*>(p) = w[0];
       }
     } else {
-      each<T>(c, [&](int i, int e) { p[e] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4))); });
+      int lo, hi;
+      inside<T>(c, lo, hi);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (i >= lo && i < hi) p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i % 4)));
+      }
     }
   }
 };
@@ -137,55 +174,29 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, int warps, fl
   }
 }
 
-// kPer chunks a thread are kept in registers; kPer = 0: rows longer than a block holds, read twice.
-// kRows > 1: a warp a row, kRows rows a block.
-template <class T, bool Q8, int kPer, int kRows>
-__global__ void __launch_bounds__(kRows > 1 ? kRows * kWarp : 1024)
-    add_rms_norm_kernel(const NormArgs a) {
+// Any row: read once for the sums and once more for the result.
+template <class T, bool Q8>
+__global__ void __launch_bounds__(1024) add_rms_norm_kernel(const NormArgs a) {
   __shared__ float2 scratch[kWarp];
   wait_then_release();
   constexpr int E = Chunk<T>::kElems;
-  const int64_t row = kRows > 1 ? static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kWarp
-                                : blockIdx.x;
-  if (kRows > 1 && row >= a.rows) return;  // whole warps: a row's warp needs no other
-  const int threads = kRows > 1 ? kWarp : blockDim.x;
-  const int tid = kRows > 1 ? threadIdx.x % kWarp : threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int64_t row0 = row * a.hidden;
   const int shift = a.aligned ? static_cast<int>(row0 % E) : 0;
   const NormRow r{a, row0, shift, (shift + a.hidden + E - 1) / E};
-
-  constexpr int kHeld = kPer > 0 ? kPer : 1;
-  Chunk<T> h[kHeld], w[kHeld];
+  Chunk<T> h, w;
   float sum = 0.0f, top = 0.0f;
-  auto add = [&](const Chunk<T>& hc, const Chunk<T>& wc) {
+  for (int c = tid; c < r.chunks; c += threads) {
+    r.load<T>(c, h);
+    if (Q8) r.load_weight<T>(c, w);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      sum = fmaf(hc.v[i], hc.v[i], sum);
-      if (Q8) top = max_nan(top, fabsf(hc.v[i] * wc.v[i]));
-    }
-  };
-  if constexpr (kPer > 0) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int c = tid + j * threads;
-      if (c < r.chunks) {
-        r.load<T>(c, h[j]);
-        r.load_weight<T>(c, w[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (tid + j * threads < r.chunks) add(h[j], w[j]);
-    }
-  } else {
-    for (int c = tid; c < r.chunks; c += threads) {
-      r.load<T>(c, h[0]);
-      if (Q8) r.load_weight<T>(c, w[0]);
-      add(h[0], w[0]);
+      sum = fmaf(h.v[i], h.v[i], sum);
+      if (Q8) top = max_nan(top, fabsf(h.v[i] * w.v[i]));
     }
   }
-  row_reduce(sum, top, kRows > 1 ? 1 : (blockDim.x + kWarp - 1) / kWarp, scratch);
-
+  row_reduce(sum, top, threads / kWarp, scratch);
   float rstd = rsqrtf(sum / static_cast<float>(a.hidden) + a.eps);
   if constexpr (Q8) {
     float scale = rstd * top / kE4m3Max;
@@ -193,75 +204,101 @@ __global__ void __launch_bounds__(kRows > 1 ? kRows * kWarp : 1024)
     if (tid == 0) a.scales[row] = scale;
     rstd = rstd / scale;
   }
-  auto finish = [&](int c, const Chunk<T>& hc, const Chunk<T>& wc) {
+  for (int c = tid; c < r.chunks; c += threads) {
+    r.load<T>(c, h);
+    r.load_weight<T>(c, w);
     Chunk<T> y;
 #pragma unroll
-    for (int i = 0; i < E; ++i) y.v[i] = hc.v[i] * rstd * wc.v[i];
-    if (a.h) r.store<T>(c, a.h, hc);
+    for (int i = 0; i < E; ++i) y.v[i] = h.v[i] * rstd * w.v[i];
+    if (a.h) r.store<T>(c, a.h, h);
     if constexpr (Q8) {
       r.store_e4m3<T>(c, y);
     } else {
       r.store<T>(c, a.y, y);
     }
-  };
-  if constexpr (kPer > 0) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int c = tid + j * threads;
-      if (c < r.chunks) finish(c, h[j], w[j]);
-    }
-  } else {
-    for (int c = tid; c < r.chunks; c += threads) {
-      r.load<T>(c, h[0]);
-      r.load_weight<T>(c, w[0]);
-      finish(c, h[0], w[0]);
-    }
   }
 }
 
-// Rows of whole chunks. kPer chunks a thread, blocks of as many threads as a row needs; rows are
-// taken in turn by the blocks of the grid.
-template <class T, bool Q8, bool kResidual, int kPer>
-__global__ void __launch_bounds__(1024) add_rms_norm_rows_kernel(const NormArgs a) {
+// Rows of aligned tensors. kPer chunks a thread, blocks of as many threads as a row needs; rows are
+// taken in turn by the blocks of the grid. kWhole: rows of whole chunks; else gridDim is a multiple
+// of a chunk's elements, or no block has more than one row.
+template <class T, bool Q8, bool kResidual, bool kWhole, int kPer>
+__global__ void __launch_bounds__(most_threads(kWhole, kPer), kPer == 2 && !kWhole ? 2 : 1)
+    add_rms_norm_rows_kernel(const NormArgs a) {
   __shared__ float2 scratch[2][kWarp];
   wait_then_release();
   constexpr int E = Chunk<T>::kElems;
-  const int chunks = a.hidden / E, tid = threadIdx.x;
-  const int warps = blockDim.x / kWarp;
-  const uint4* x = static_cast<const uint4*>(a.x);
-  const uint4* residual = static_cast<const uint4*>(a.residual);
-  const uint4* weight = static_cast<const uint4*>(a.weight);
+  const int tid = threadIdx.x, warps = blockDim.x / kWarp;
+  int64_t row = blockIdx.x;
+  const int shift = kWhole ? 0 : static_cast<int>(row * a.hidden % E);
+  const int chunks = (shift + a.hidden + E - 1) / E;
+  const T* weight = static_cast<const T*>(a.weight);
+  // elements of chunk c outside of the row
+  auto outside = [&](int c, int i) {
+    const int e = c * E - shift + i;
+    return !kWhole && (e < 0 || e >= a.hidden);
+  };
+  auto whole = [&](int c) { return kWhole || (c * E >= shift && c * E - shift + E <= a.hidden); };
 
   uint4 w[kPer], nx[kPer], nr[kPer];
   auto fetch = [&](int64_t row) {
+    const int64_t at = row * a.hidden - shift;  // of the first chunk
+    const T* x = static_cast<const T*>(a.x) + at;
+    const T* residual = static_cast<const T*>(a.residual) + at;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int c = tid + j * blockDim.x;
-      if (c < chunks) {
-        nx[j] = ld_stream_v4(x + row * chunks + c);
-        if (kResidual) nr[j] = ld_stream_v4(residual + row * chunks + c);
+      if (c >= chunks) continue;
+      if (kWhole || row + 1 < a.rows || whole(c)) {
+        // what a chunk holds of a neighbouring row is read, and left out of the sum
+        nx[j] = ld_stream_v4(x + c * E);
+        if (kResidual) nr[j] = ld_stream_v4(residual + c * E);
+      } else {  // the tensors may end inside of the last chunk
+        Chunk<T> fx, fr;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          fx.v[i] = outside(c, i) ? 0.0f : to_f32(x[c * E + i]);
+          fr.v[i] = outside(c, i) || !kResidual ? 0.0f : to_f32(residual[c * E + i]);
+        }
+        nx[j] = fx.get();
+        nr[j] = fr.get();
       }
     }
   };
-  int64_t row = blockIdx.x;
   fetch(row);
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int c = tid + j * blockDim.x;
-    w[j] = c < chunks ? weight[c] : make_uint4(0, 0, 0, 0);
+    Chunk<T> f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) f.v[i] = 0.0f;
+    if (kWhole) {
+      if (c < chunks) f.set(*reinterpret_cast<const uint4*>(weight + c * E));
+    } else if (c < chunks) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (!outside(c, i)) f.v[i] = to_f32(weight[c * E - shift + i]);
+      }
+    }
+    w[j] = f.get();
   }
   for (int turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
     Chunk<T> h[kPer];
     float sum = 0.0f, top = 0.0f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      if (tid + j * static_cast<int>(blockDim.x) >= chunks) continue;
+      const int c = tid + j * static_cast<int>(blockDim.x);
+      if (c >= chunks) continue;
       h[j].set(nx[j]);
       if (kResidual) {
         Chunk<T> r;
         r.set(nr[j]);
 #pragma unroll
         for (int i = 0; i < E; ++i) h[j].v[i] += r.v[i];
+      }
+      if (!whole(c)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) h[j].v[i] = outside(c, i) ? 0.0f : h[j].v[i];
       }
       Chunk<T> wc;
       if (Q8) wc.set(w[j]);
@@ -281,25 +318,20 @@ __global__ void __launch_bounds__(1024) add_rms_norm_rows_kernel(const NormArgs 
       if (tid == 0) a.scales[row] = scale;
       rstd = rstd / scale;
     }
+    const NormRow r{a, row * a.hidden, shift, chunks};
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int c = tid + j * blockDim.x;
       if (c >= chunks) continue;
-      if (kResidual) static_cast<uint4*>(a.h)[row * chunks + c] = h[j].get();
+      if (kResidual) r.store<T, kWhole>(c, a.h, h[j]);
       Chunk<T> y;
       y.set(w[j]);
 #pragma unroll
       for (int i = 0; i < E; ++i) y.v[i] = h[j].v[i] * rstd * y.v[i];
-      if constexpr (!Q8) {
-        static_cast<uint4*>(a.y)[row * chunks + c] = y.get();
+      if constexpr (Q8) {
+        r.store_e4m3<T, kWhole>(c, y);
       } else {
-        uint32_t* to = static_cast<uint32_t*>(a.y) + (row * chunks + c) * (E / 4);
-        if constexpr (E == 8) {
-          *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(y.v[0], y.v[1], y.v[2], y.v[3]),
-                                                     e4m3x4(y.v[4], y.v[5], y.v[6], y.v[7]));
-        } else {
-          *to = e4m3x4(y.v[0], y.v[1], y.v[2], y.v[3]);
-        }
+        r.store<T, kWhole>(c, a.y, y);
       }
     }
   }
@@ -309,36 +341,33 @@ template <class T, bool Q8>
 cudaError_t launch(const NormArgs& a, cudaStream_t stream) {
   constexpr int E = Chunk<T>::kElems;
   const auto up = [](int n, int to) { return (n + to - 1) / to * to; };
-  // without a residual h is x, and a caller that asks for it gets a copy from the general kernel
-  if (a.aligned && a.hidden % E == 0 && a.hidden / E <= 2048 && (a.residual || !a.h)) {
-    const int chunks = a.hidden / E;
-    const auto rows = [&](auto with, auto without, int per) {
-      const int threads = up((chunks + per - 1) / per, kWarp);
-      const int ctas = std::max(1, kRowThreads / threads) * sm_count();
-      return launch_serialised(a.residual ? with : without, dim3(std::min(a.rows, ctas)),
-                               dim3(threads), 0, stream, 1, a);
-    };
-    const bool few = a.rows <= sm_count();
-    if (chunks <= 256 || (few && chunks <= 1024)) {
-      return rows(add_rms_norm_rows_kernel<T, Q8, true, 1>, add_rms_norm_rows_kernel<T, Q8, false, 1>, 1);
-    }
-    return rows(add_rms_norm_rows_kernel<T, Q8, true, 2>, add_rms_norm_rows_kernel<T, Q8, false, 2>, 2);
+  const bool whole = a.hidden % E == 0;
+  const int chunks = whole ? a.hidden / E : (E - 1 + a.hidden + E - 1) / E;  // at any shift
+  // without a residual h is x, and a caller that asks for it gets a copy from the plain loop
+  if (!a.aligned || chunks > (whole ? 2 * 1024 : 3 * most_threads(false, 3)) || (a.h && !a.residual)) {
+    return launch_serialised(add_rms_norm_kernel<T, Q8>, dim3(a.rows),
+                             dim3(std::min(1024, up(chunks, kWarp))), 0, stream, 1, a);
   }
-  const int most = (E - 1 + a.hidden + E - 1) / E;  // chunks of a row at any shift
-  if (most <= kWarp * 4 && a.rows > 1) {
-    constexpr int kRows = 4;
-    return launch_serialised(add_rms_norm_kernel<T, Q8, 4, kRows>,
-                             dim3((a.rows + kRows - 1) / kRows), dim3(kRows * kWarp), 0, stream, 1,
-                             a);
-  }
-  const auto block = [&](auto kernel, int per) {
-    return launch_serialised(kernel, dim3(a.rows), dim3(up((most + per - 1) / per, kWarp)), 0,
-                             stream, 1, a);
+  // one chunk a thread for rows of few chunks, and for few rows (latency); else two, or three
+  const int per = chunks <= 256 || (a.rows <= sm_count() && chunks <= 1024) ? 1
+                  : chunks <= 2 * most_threads(whole, 2)                    ? 2
+                                                                            : 3;
+  const int threads = up((chunks + per - 1) / per, kWarp);
+  int ctas = (threads > 512 ? (threads <= most_threads(false, 2) ? 2 : 1) : kRowThreads / threads) * sm_count();
+  if (!whole) ctas = ctas / E * E;
+  const auto rows = [&](auto one, auto two, auto three) {
+    return launch_serialised(per == 1 ? one : per == 2 ? two : three, dim3(std::min(a.rows, ctas)),
+                             dim3(threads), 0, stream, 1, a);
   };
-  if (most <= 1024) return block(add_rms_norm_kernel<T, Q8, 1, 1>, 1);
-  if (most <= 2048) return block(add_rms_norm_kernel<T, Q8, 2, 1>, 2);
-  return launch_serialised(add_rms_norm_kernel<T, Q8, 0, 1>, dim3(a.rows), dim3(1024), 0, stream, 1,
-                           a);
+  const auto kind = [&]<bool kResidual, bool kWhole>() {
+    return rows(add_rms_norm_rows_kernel<T, Q8, kResidual, kWhole, 1>,
+                add_rms_norm_rows_kernel<T, Q8, kResidual, kWhole, 2>,
+                add_rms_norm_rows_kernel<T, Q8, kResidual, kWhole, kWhole ? 2 : 3>);
+  };
+  if (a.residual) {
+    return whole ? kind.template operator()<true, true>() : kind.template operator()<true, false>();
+  }
+  return whole ? kind.template operator()<false, true>() : kind.template operator()<false, false>();
 }
 
 template <bool Q8>
