@@ -215,18 +215,30 @@ def check_attention(c, hq, dtype, append, weights, scale=None):
 LENS = [1, 0, 15, 16, 17, 63, 64, 65, 200, 333]
 
 
-@pytest.mark.parametrize("group,hkv,dim,page,layout", [
+SHAPES = [
     (4, 2, 128, 16, "tokens"), (4, 2, 128, 16, "heads"), (8, 2, 128, 32, "pairs"),
     (1, 3, 64, 16, "tokens"), (2, 1, 64, 8, "heads"), (3, 2, 80, 48, "pairs"),
     (7, 1, 96, 64, "tokens"), (16, 2, 128, 128, "heads"), (17, 1, 64, 16, "tokens"),
     (40, 1, 128, 16, "pairs"), (5, 2, 256, 16, "tokens"), (16, 1, 192, 24, "heads"),
     (4, 2, 8, 1, "tokens"), (6, 2, 40, 5, "heads"), (33, 1, 136, 256, "tokens"),
-])
+]
+
+
+@pytest.mark.parametrize("group,hkv,dim,page,layout", SHAPES)
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attention(group, hkv, dim, page, layout, dtype):
     for append, weights in ((False, False), (True, True)):
         c = Paged(LENS, hkv, dim, page, dtype, seed=group * dim, layout=layout, width=400)
         check_attention(c, group * hkv, dtype, append, weights)
+
+
+@pytest.mark.parametrize("group,hkv,dim,page,layout", SHAPES)
+def test_attention_of_narrow_and_wide_tables(group, hkv, dim, page, layout):
+    """The same call by the kernel for small calls (a narrow table, few sequences) and by the one for
+    any call (a table too wide for it), each with new tokens and weights."""
+    for width in (-(-333 // page), 60000 // page):
+        c = Paged([333, 0, 64, 65], hkv, dim, page, F16, seed=dim + page, layout=layout, width=width)
+        check_attention(c, group * hkv, F16, True, True)
 
 
 @pytest.mark.parametrize("lens,group,hkv,dim", [
@@ -265,10 +277,11 @@ def test_attention_is_deterministic_and_takes_views():
         assert same_bits(first, ops.paged_attention(q, c.k, c.v, c.table, c.seq_lens, 0.1))
 
 
-def test_bad_pages_and_lengths_are_reported():
+@pytest.mark.parametrize("width", [7, 5000])
+def test_bad_pages_and_lengths_are_reported(width):
     """A page outside of the cache is left out, a length the table has no room for clamped: the
     status says so, other sequences and everything outside of the call's places stay as they were."""
-    c = Paged([100, 80, 64], 2, 64, 16, F16, seed=4, width=7)
+    c = Paged([100, 80, 64], 2, 64, 16, F16, seed=4, width=width)
     q = randn(c.g, 3, 4, 64, dtype=F16)
     good = ops.paged_attention(q, c.k, c.v, c.table, c.seq_lens, 0.125)
     k0, v0, w0 = c.k.clone(), c.v.clone(), c.weights.clone()
@@ -293,7 +306,7 @@ def test_bad_pages_and_lengths_are_reported():
 
     lens = torch.tensor([10**6, -3, 64], dtype=torch.int32, device="cuda")
     full = c.table.clone()
-    full[0] = c.table[0, 0]  # seven times the same page: 112 positions
+    full[0] = c.table[0, 0]  # the same page again and again
     out = ops.paged_attention(q, c.k, c.v, full, lens, 0.125)
     assert capi.device_status() == capi.STATUS_BAD_PAGE
     assert (out[1] == 0).all() and same_bits(out[2], good[2]) and out[0].isfinite().all()
@@ -543,6 +556,8 @@ def test_logprobs_special_rows(dtype):
     check_logprobs(x, tokens, top)
     check_logprobs(x, tokens, 0)
     check_logprobs(x, tokens, 32)
+    # many rows, of which a block takes one after the other
+    check_logprobs(x.repeat(60, 1), tokens.repeat(60), 17)
 
 
 def test_logprobs_tokens_outside_and_views():
