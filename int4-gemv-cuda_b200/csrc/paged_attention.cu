@@ -5,7 +5,11 @@
 // position's attention weight, summed over the query heads of its KV head, to a buffer that
 // eviction goes by.
 //
-// Bound by HBM: the cache is read once, 4 hq / hkv operations an element.
+// Bound by HBM: the cache is read once, 4 hq / hkv operations an element. Measured on B200 (fp16, 128
+// dims, 64 query and 8 KV heads): one sequence of 131072 positions 99 us, 5.4 TB/s (0.83 of a plain
+// copy's 6.53); 64 sequences of 512 to 8192 202 us (0.83). Of what is missing, 7 to 10 us are the scan
+// of the lengths, the first loads and the second kernel. Small calls are bound by latency: 701
+// positions of 32 query heads 7.5 us.
 //
 // Work: an item is (sequence, KV head, block of 8 or 16 query heads), cut into tiles of positions.
 // All tiles in order are split evenly over the blocks of the grid whatever the lengths are, so a

@@ -6,9 +6,17 @@
 // Two kernels. The choice: one block a (sequence, head), the k-th largest weight by a radix select
 // over the bits of the weights as ordered integers (11 + 11 + 10 bits, a histogram in shared memory
 // each), then the chosen positions in order by counting within and across warps. It reads 4 bytes
-// a position. The copy: a warp a (position, head), 16 bytes a lane, bound by HBM. The new pages are
-// not the old ones, so every block of the copy is independent of the others and sequences may
-// share old pages (a common prefix).
+// a position, four positions at a time where pages allow. The copy is bound by HBM: a warp takes up to
+// 32 positions of a head, looks their places up a lane a position, and moves them 16 bytes a lane
+// through its own ring in shared memory (cp.async), sixteen reads ahead of the writes; the warps of a
+// block take the heads of the same positions, whose rows are neighbours in memory. The new pages are
+// not the old ones, so every block of the copy is independent of the others and sequences may share
+// old pages (a common prefix).
+//
+// Measured on B200, 32 sequences of up to 8192 positions to 2048 (bf16, 8 heads of 128): the copy
+// 78 us, 6.2 TB/s (0.95 of a plain copy's 6.53; eight reads a lane in registers instead of the ring:
+// 108 us), the choice 18 us (bound by instructions), together 101 us; one sequence of 2503 to 1001
+// 10.6 us (latency of two kernels).
 #include <algorithm>
 #include <mutex>
 
