@@ -8,8 +8,8 @@
 // Bound by HBM: the cache is read once, 4 hq / hkv operations an element. Measured on B200 (fp16, 128
 // dims, 64 query and 8 KV heads): one sequence of 131072 positions 99 us, 5.4 TB/s (0.83 of a plain
 // copy's 6.53); 64 sequences of 512 to 8192 202 us (0.83). Of what is missing, 7 to 10 us are the scan
-// of the lengths, the first loads and the second kernel. Small calls are bound by latency: 701
-// positions of 32 query heads 7.5 us.
+// of the lengths, the first loads and the second kernel. Weights cost 7 us more at 24 sequences of up to
+// 4096 (48 to 55 us). Small calls are bound by latency: 701 positions of 32 query heads 7.5 us.
 //
 // Work: an item is (sequence, KV head, block of 8 or 16 query heads), cut into tiles of positions.
 // All tiles in order are split evenly over the blocks of the grid whatever the lengths are, so a
@@ -444,43 +444,64 @@ struct Sums {
 
 // By a block of kThreads: adds the weights of `positions` positions of KV head kv of sequence b (n
 // long), from tile `tile0` of the sequence on, whose scores begin at tile `scores_tile`, for one item
-// (block `ht` of the head's query heads) whose rows have the sums row_lse.
-template <int kThreads>
+// (block `ht` of the head's query heads) whose rows have the sums row_lse. `ready` (by all threads, if
+// there are positions) sees to those while the first loads are on their way.
+template <int kThreads, class F>
 __device__ __forceinline__ void add_weights(const Plan& p, int b, int kv, int ht, int rows,
                                             int scores_tile, int tile0, int positions, int n,
-                                            const float* row_lse) {
-  constexpr int kAtOnce = 2;
+                                            const float* row_lse, F ready) {
+  constexpr int kAtOnce = 2, kFirst = 2;  // positions of a thread; pairs of rows loaded before `ready`
   const PagedAttentionArgs& a = p.a;
   const PagedCache& c = a.cache;
-  for (int i0 = threadIdx.x; i0 < positions; i0 += kAtOnce * kThreads) {
+  for (int i0 = 0; i0 < positions; i0 += kAtOnce * kThreads) {
     float* to[kAtOnce];
+    float2 v[kAtOnce][kFirst];
     float w[kAtOnce];
+    int page[kAtOnce];
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      const int i = i0 + k * kThreads, pos = tile0 * p.tile + i;
-      to[k] = nullptr;
-      w[k] = 0.0f;
+      const int i = i0 + k * kThreads + static_cast<int>(threadIdx.x);
+      page[k] = -1;
       if (i >= positions) continue;
-      const int block = p.page.quotient(pos);
-      const int page = a.table[static_cast<int64_t>(b) * a.max_blocks + block];
+      page[k] = a.table[static_cast<int64_t>(b) * a.max_blocks + p.page.quotient(tile0 * p.tile + i)];
       const float2* s = reinterpret_cast<const float2*>(
           p.scores + (static_cast<int64_t>(scores_tile) * p.tile + i) * p.score_rows);
-#pragma unroll 4
-      for (int r = 0; r < rows; r += 2) {
-        const float2 v = s[r / 2];
-        w[k] += exp2_fast(v.x - row_lse[r]);
-        if (r + 1 < rows) w[k] += exp2_fast(v.y - row_lse[r + 1]);
-      }
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
-        to[k] = c.weights + (static_cast<int64_t>(page) * c.hkv + kv) * c.block_size +
-                (pos - block * static_cast<int>(p.page.by));
-        // a new token's slot may hold what its page was used for before
-        if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] += *to[k];
+#pragma unroll
+      for (int r = 0; r < kFirst; ++r) {
+        if (2 * r < rows) v[k][r] = s[r];
       }
     }
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
-      if (to[k]) *to[k] = w[k];
+      const int pos = tile0 * p.tile + i0 + k * kThreads + static_cast<int>(threadIdx.x);
+      to[k] = nullptr;
+      w[k] = 0.0f;
+      if (static_cast<unsigned>(page[k]) >= static_cast<unsigned>(c.num_blocks)) continue;
+      to[k] = c.weights + (static_cast<int64_t>(page[k]) * c.hkv + kv) * c.block_size +
+              (pos - p.page.quotient(pos) * static_cast<int>(p.page.by));
+      // a new token's slot may hold what its page was used for before
+      if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] = *to[k];
+    }
+    if (i0 == 0) ready();
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (!to[k]) continue;
+      const int i = i0 + k * kThreads + static_cast<int>(threadIdx.x);
+      const float2* s = reinterpret_cast<const float2*>(
+          p.scores + (static_cast<int64_t>(scores_tile) * p.tile + i) * p.score_rows);
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < kFirst; ++r) {
+        if (2 * r < rows) sum += exp2_fast(v[k][r].x - row_lse[2 * r]);
+        if (2 * r + 1 < rows) sum += exp2_fast(v[k][r].y - row_lse[2 * r + 1]);
+      }
+#pragma unroll 2
+      for (int r = kFirst; 2 * r < rows; ++r) {
+        const float2 more = s[r];
+        sum += exp2_fast(more.x - row_lse[2 * r]);
+        if (2 * r + 1 < rows) sum += exp2_fast(more.y - row_lse[2 * r + 1]);
+      }
+      *to[k] = w[k] + sum;
     }
   }
 }
@@ -849,7 +870,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
     for (int i = 0; i < own; ++i) {
       const int tile = rank + i * ranks;
       add_weights<kThreads>(p, b, kv, 0, rows, index * p.item_tiles + tile, tile,
-                            min(kTile, n - tile * kTile), n, sh.row_lse);
+                            min(kTile, n - tile * kTile), n, sh.row_lse, [] {});
     }
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -864,6 +885,10 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
 // positions at a time.
 constexpr int kJoinThreads = 128;
 constexpr int kJoinWarps = kJoinThreads / kWarp;
+// Blocks an SM that also adds weights, in one wave: their chain of loads is the time, so all start at
+// once. 24 sequences of up to 4096: 55.0 us with 6 (80 registers), 56 with 5; 57.7 with 8 and 62.5 with
+// 10, which spill; 64.3 with four parts at a time and no bound (120 registers, three waves).
+constexpr int kJoinCtas = 6;
 
 // Reads of the attention kernel's workspace
 struct Parts {
@@ -895,7 +920,7 @@ struct Parts {
   }
 };
 
-template <class T>
+template <class T, int kAtOnce>
 __device__ __forceinline__ void join_head(const Plan& p) {
   __shared__ alignas(16) float sums[kJoinWarps][kMaxDim];
   const PagedAttentionArgs& a = p.a;
@@ -916,7 +941,6 @@ __device__ __forceinline__ void join_head(const Plan& p) {
   }
   const Parts parts(p, p.first_tile[a.batch], first + item * tiles, tiles);
   if (parts.count == 1) return;
-  constexpr int kAtOnce = 4;
   float2 ml = make_float2(0.0f, 0.0f);
   float4 v[2] = {};
   for (int i0 = sub; i0 < parts.count; i0 += kAtOnce * p.join_warps) {
@@ -1010,19 +1034,21 @@ __device__ __forceinline__ void join_weights(const Plan& p, int block, int block
       const int begin = p.first_tile[b] + (kv * p.head_tiles + ht) * tiles;
       const int rows = min(p.group - ht * p.rows, p.rows);
       const Parts parts(p, total, begin, tiles);
-      if (parts.count == 1) {
-        if (tid < rows) {
-          row_lse[tid] = p.lse[static_cast<int64_t>(b) * a.hq + kv * p.group + ht * p.rows + tid];
-        }
-      } else {
-        for (int r = warp; r < rows; r += kJoinWarps) {
-          const float2 ml = parts.row(r, lane);
-          if (lane == 0) row_lse[r] = ml.x + log2f(ml.y);
-        }
-      }
-      __syncthreads();
-      add_weights<kJoinThreads>(p, b, kv, ht, rows, begin + tile0, tile0,
-                                min(count * p.tile, n - tile0 * p.tile), n, row_lse);
+      add_weights<kJoinThreads>(
+          p, b, kv, ht, rows, begin + tile0, tile0, min(count * p.tile, n - tile0 * p.tile), n, row_lse,
+          [&] {
+            if (parts.count == 1) {
+              if (tid < rows) {
+                row_lse[tid] = p.lse[static_cast<int64_t>(b) * a.hq + kv * p.group + ht * p.rows + tid];
+              }
+            } else {
+              for (int r = warp; r < rows; r += kJoinWarps) {
+                const float2 ml = parts.row(r, lane);
+                if (lane == 0) row_lse[r] = ml.x + log2f(ml.y);
+              }
+            }
+            __syncthreads();
+          });
       __syncthreads();  // row_lse is rewritten
     }
     t += count;
@@ -1030,10 +1056,11 @@ __device__ __forceinline__ void join_weights(const Plan& p, int block, int block
 }
 
 template <class T, bool kWeights>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ Plan p) {
+__global__ void __launch_bounds__(kJoinThreads, kWeights ? kJoinCtas : 1)
+paged_join_kernel(const __grid_constant__ Plan p) {
   wait_then_release();
   if (static_cast<int>(blockIdx.x) < p.join_blocks) {
-    join_head<T>(p);
+    join_head<T, kWeights ? 2 : 4>(p);
   } else if constexpr (kWeights) {
     join_weights(p, blockIdx.x - p.join_blocks, gridDim.x - p.join_blocks);
   }
@@ -1146,9 +1173,10 @@ cudaError_t launch(const Plan& p, cudaStream_t stream) {
   err = launch_serialised(paged_attention_kernel<T, DP, NT, kWeights>, dim3(p.blocks),
                           dim3(Shape<DP, NT, false>::kThreads), sizeof(Smem<DP, NT>), stream, 1, p);
   if (err != cudaSuccess) return err;
-  return launch_serialised(paged_join_kernel<T, kWeights>,
-                           dim3(p.join_blocks + (kWeights ? 8 * sm_count() : 0)),
-                           dim3(kJoinThreads), 0, stream, 1, p);
+  const int blocks = kWeights ? std::max(kJoinCtas * sm_count(), p.join_blocks + sm_count())
+                              : p.join_blocks;
+  return launch_serialised(paged_join_kernel<T, kWeights>, dim3(blocks), dim3(kJoinThreads), 0, stream,
+                           1, p);
 }
 
 }  // namespace
