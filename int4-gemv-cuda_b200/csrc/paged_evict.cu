@@ -9,8 +9,9 @@
 // a position, four positions at a time where pages allow. The copy is bound by HBM: a warp takes up to
 // 32 positions of a head, looks their places up a lane a position, and moves them 16 bytes a lane
 // through its own ring in shared memory (cp.async), sixteen reads ahead of the writes; the warps of a
-// block take the heads of the same positions, whose rows are neighbours in memory. The new pages are
-// not the old ones, so every block of the copy is independent of the others and sequences may share
+// block take the heads of the same positions, whose rows are neighbours in memory; where the heads are
+// fewer than the warps, several warps take a head (13 sequences of up to 20204 to 9886, 2 heads of 64:
+// copy 25 us, without that 48). The new pages are not the old ones, so every block of the copy is independent of the others and sequences may share
 // old pages (a common prefix).
 //
 // Measured on B200, 32 sequences of up to 8192 positions to 2048 (bf16, 8 heads of 128): the copy
@@ -226,17 +227,19 @@ constexpr int kCopyWarps = kCopyThreads / kWarp;
 constexpr int kDepth = 16;  // 16-byte pieces a lane has in flight
 constexpr int kCopySmem = kCopyWarps * kDepth * kWarp * 16;
 
-// `span` positions a warp, at most 32.
+// `span` positions a warp, at most 32; with few heads `groups` warps a head, each with its positions.
 __global__ void __launch_bounds__(kCopyThreads)
-    evict_copy_kernel(const PagedEvictArgs a, const Divider by_page, int span, int* status) {
+    evict_copy_kernel(const PagedEvictArgs a, const Divider by_page, int span, int groups,
+                      int* status) {
   extern __shared__ __align__(16) unsigned char ring_raw[];
   wait_then_release();
   const PagedCache& c = a.cache;
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int b = blockIdx.y;
   const int kept = a.new_lens[b];
-  const int j0 = blockIdx.x * span;
-  if (j0 >= kept) return;
+  const int group = groups > 1 ? warp / c.hkv : 0;
+  const int j0 = (blockIdx.x * groups + group) * span;
+  if (group >= groups || j0 >= kept) return;
   const int* table = a.table + static_cast<int64_t>(b) * a.max_blocks;
   const int* new_table = a.new_table + static_cast<int64_t>(b) * a.new_blocks;
   const int vectors = c.dim / 8;  // 16-byte pieces of a row of keys
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kCopyThreads)
   const int count = min(span, kept - j0);
   const uint32_t ring = smem_addr(ring_raw) + (warp * kDepth * kWarp + lane) * 16;
 
-  for (int h = warp; h < c.hkv; h += kCopyWarps) {
+  for (int h = warp - group * c.hkv; h < c.hkv; h += kCopyWarps) {
     // this lane's position: where it is and where it goes
     int from_page = -1, from_off = 0, to_page = -1, to_off = 0;
     if (lane < count) {
@@ -324,12 +327,13 @@ cudaError_t launch_paged_evict(const PagedEvictArgs& a, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const int64_t longest = a.budget < most ? a.budget : most;
   if (longest == 0) return cudaSuccess;
+  const int groups = std::max(1, kCopyWarps / a.cache.hkv);
   // 32 positions a warp where that gives every SM three blocks, down to 8 where it does not
+  auto blocks = [&](int span) { return (longest + span * groups - 1) / (span * groups); };
   int span = kWarp;
-  while (span > 8 && (longest + span - 1) / span * a.batch < 3 * sm_count()) span /= 2;
-  return launch_serialised(evict_copy_kernel,
-                           dim3(static_cast<unsigned>((longest + span - 1) / span), a.batch),
-                           dim3(kCopyThreads), kCopySmem, stream, 1, a, by_page, span, status);
+  while (span > 8 && blocks(span) * a.batch < 3 * sm_count()) span /= 2;
+  return launch_serialised(evict_copy_kernel, dim3(static_cast<unsigned>(blocks(span)), a.batch),
+                           dim3(kCopyThreads), kCopySmem, stream, 1, a, by_page, span, groups, status);
 }
 
 }  // namespace i4

@@ -422,7 +422,8 @@ def test_evict(budget, recent, layout):
 
 
 @pytest.mark.parametrize("dim,page,hkv,dtype", [(8, 1, 1, F16), (80, 48, 2, BF16), (256, 8, 2, F16),
-                                                (136, 7, 5, BF16)])
+                                                (136, 7, 5, BF16), (64, 16, 4, F16), (128, 32, 8, BF16),
+                                                (72, 16, 12, F16)])
 def test_evict_shapes(dim, page, hkv, dtype):
     check_evict(Paged([200, 77, 30], hkv, dim, page, dtype, seed=dim, spare=400), 60, 20)
 
