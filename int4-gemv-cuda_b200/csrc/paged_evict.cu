@@ -11,8 +11,8 @@
 // through its own ring in shared memory (cp.async), sixteen reads ahead of the writes; the warps of a
 // block take the heads of the same positions, whose rows are neighbours in memory; where the heads are
 // fewer than the warps, several warps take a head (13 sequences of up to 20204 to 9886, 2 heads of 64:
-// copy 25 us, without that 48). The new pages are not the old ones, so every block of the copy is independent of the others and sequences may share
-// old pages (a common prefix).
+// copy 25 us, without that 48). The new pages are not the old ones, so every block of the copy is
+// independent of the others and sequences may share old pages (a common prefix).
 //
 // Measured on B200, 32 sequences of up to 8192 positions to 2048 (bf16, 8 heads of 128): the copy
 // 78 us, 6.2 TB/s (0.95 of a plain copy's 6.53; eight reads a lane in registers instead of the ring:
