@@ -247,15 +247,17 @@ __global__ void __launch_bounds__(most_threads(kWhole, kPer), kPer == 2 && !kWho
     const int64_t at = row * a.hidden - shift;  // of the first chunk
     const T* x = static_cast<const T*>(a.x) + at;
     const T* residual = static_cast<const T*>(a.residual) + at;
+    const int64_t left = static_cast<int64_t>(a.rows) * a.hidden - at;  // elements up to the tensors' end
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int c = tid + j * blockDim.x;
       if (c >= chunks) continue;
-      if (kWhole || row + 1 < a.rows || whole(c)) {
-        // what a chunk holds of a neighbouring row is read, and left out of the sum
+      if (kWhole || (c + 1) * E <= left) {
+        // what a chunk holds of neighbouring rows (several, where they are shorter than a chunk) is
+        // read, and left out of the sum
         nx[j] = ld_stream_v4(x + c * E);
         if (kResidual) nr[j] = ld_stream_v4(residual + c * E);
-      } else {  // the tensors may end inside of the last chunk
+      } else {  // the tensors end inside of the last chunk
         Chunk<T> fx, fr;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
