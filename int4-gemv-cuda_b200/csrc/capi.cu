@@ -1060,11 +1060,14 @@ int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_
                 name, static_cast<long long>(new_blocks * cache->block_size),
                 static_cast<long long>(budget));
   }
-  if (max_blocks * cache->block_size > INT_MAX || batch * cache->kv_heads > INT_MAX ||
-      budget * cache->kv_heads / 8 > INT_MAX) {
-    return fail(INT4GEMV_ERR_INVALID, "%s: batch = %lld with tables of %lld blocks of %lld is out of range",
+  // the kernels' loops step past the last position by less than this, in 32 bits
+  constexpr int64_t kMostPositions = INT_MAX - 8192;
+  if (budget > kMostPositions || max_blocks * cache->block_size > kMostPositions ||
+      batch * cache->kv_heads > INT_MAX || budget * cache->kv_heads / 8 > INT_MAX) {
+    return fail(INT4GEMV_ERR_INVALID,
+                "%s: batch = %lld with tables of %lld blocks of %lld and a budget of %lld is out of range",
                 name, static_cast<long long>(batch), static_cast<long long>(max_blocks),
-                static_cast<long long>(cache->block_size));
+                static_cast<long long>(cache->block_size), static_cast<long long>(budget));
   }
   if (batch == 0) return ok();
   const bool some_pages = cache->num_blocks > 0;
