@@ -311,8 +311,8 @@ int int4gemv_w4a16_exchange_static(void* y, const void* x, const void* qweight,
  *   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight,
  * computed in fp32 from the unrounded sum; h and y are rounded once. x, residual, weight [hidden],
  * h and y have one element type, dtype (INT4GEMV_DTYPE_F32, _F16 or _BF16). residual may be NULL (h = x);
- * h may then be NULL too, and is not written. h may be x or residual itself. Any hidden >= 1;
- * fastest when all pointers are 16-byte aligned. */
+ * h may then be NULL too, and is not written. h may be x or residual itself; y overlaps no other
+ * tensor of the call. Any hidden >= 1; fastest when all pointers are 16-byte aligned. */
 int int4gemv_add_rms_norm(void* y, void* h, const void* x, const void* residual, const void* weight,
                           float eps, int dtype, int64_t rows, int64_t hidden, void* stream);
 
@@ -346,6 +346,7 @@ size_t int4gemv_paged_cache_struct_bytes(void);
 /* Attention of one new token a sequence: out [batch, q_heads, head_dim] =
  * softmax(scale q k^T) v over positions [0, seq_lens[b]) of sequence b, query head h reading KV
  * head h / (q_heads / kv_heads); q and out have the cache's type, the softmax and the sums are fp32.
+ * q, out, k_new and v_new are 16-byte aligned, and out does not overlap q.
  * A sequence of length 0 gives zeros. block_table [batch, max_blocks] and seq_lens [batch] are
  * int32; table entries behind a sequence's last page are not read.
  * k_new, v_new ([batch, kv_heads, head_dim], or both NULL): the new token's key and value. seq_lens
@@ -377,8 +378,8 @@ int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* ca
  * positions 0, 1, ... of the pages in new_table [batch, new_blocks]; new_lens [batch] =
  * min(n, budget); kept [batch, kv_heads, budget] holds the old positions, then -1. Heads choose
  * for themselves: afterwards position j of two heads may come from different tokens. The new pages
- * must not be among the old ones, nor be named twice; the old pages are left as they were, so
- * sequences may share them. Lengths and pages outside of the cache are treated as in
+ * must not be among the old ones, nor be named twice, and new_lens and kept overlap no input; the
+ * old pages are left as they were, so sequences may share them. Lengths and pages outside of the cache are treated as in
  * int4gemv_paged_attention (an unreadable weight counts as lowest, an unreadable page is not copied). */
 int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_cache_t* cache,
                          const int32_t* block_table, const int32_t* seq_lens,

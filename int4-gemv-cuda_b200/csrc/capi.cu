@@ -271,6 +271,9 @@ int run_norm(const char* name, i4::NormArgs a, int dtype, int64_t rows, int64_t 
   if (!aligned_to(a.y, a.scales ? 1 : size) || !aligned_to(a.scales, 4)) {
     return fail(INT4GEMV_ERR_INVALID, "%s: y and scales must be aligned to an element", name);
   }
+  if (a.y == a.h || (a.scales && (a.y == a.x || a.y == a.residual))) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: y must not be h, nor x or residual where it is of 8 bits", name);
+  }
   a.rows = static_cast<int>(rows);
   a.hidden = static_cast<int>(hidden);
   a.aligned = aligned_to(a.x, 16) && aligned_to(a.residual, 16) && aligned_to(a.weight, 16) &&
@@ -1029,6 +1032,8 @@ int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cach
     return fail(INT4GEMV_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %lld bytes is needed, got %lld",
                 name, static_cast<long long>(bytes), static_cast<long long>(workspace ? workspace_bytes : 0));
   }
+  // blocks that share a sequence read q at different times
+  if (out == q) return fail(INT4GEMV_ERR_INVALID, "%s: out must not be q", name);
   // a flag for the kernel: weights are added where the pointer is set
   if (add_weights && !some_pages) a.cache.weights = reinterpret_cast<float*>(out);
   if (!some_pages) a.cache.k = a.cache.v = const_cast<void*>(q);  // an address that is not read
@@ -1074,6 +1079,10 @@ int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_
   if (!kept || !new_lens || !seq_lens || (max_blocks > 0 && !block_table) || !new_table ||
       (some_pages && (!cache->k || !cache->v || !cache->weights))) {
     return fail(INT4GEMV_ERR_INVALID, "%s: null pointer for a non-empty tensor", name);
+  }
+  // every head reads seq_lens while the first one writes new_lens; new pages are not old ones
+  if (new_lens == seq_lens || new_table == block_table) {
+    return fail(INT4GEMV_ERR_INVALID, "%s: new_lens must not be seq_lens, nor new_table block_table", name);
   }
   i4::PagedEvictArgs a{make_cache(cache, true), block_table, seq_lens, new_table, kept, new_lens,
                        static_cast<int>(batch), static_cast<int>(max_blocks),

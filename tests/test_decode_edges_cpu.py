@@ -18,3 +18,22 @@ def test_evict_refuses_positions_near_the_end_of_32_bits(block_size, max_blocks,
     message = refused("int4gemv_paged_evict", FAKE, FAKE, ctypes.addressof(c), FAKE, FAKE, FAKE, budget, 4,
                       1, max_blocks, new_blocks, None)
     assert message.startswith("paged_evict: batch = 1 with tables of") and message.endswith("out of range")
+
+
+def test_the_same_tensor_twice_is_refused():
+    """Outputs in the place of tensors that other blocks still read."""
+    other = FAKE * 2
+    for y, h, x, residual in ((FAKE, FAKE, other, other), (other, other, other, None)):
+        assert refused("int4gemv_add_rms_norm", y, h, x, residual, FAKE * 3, 1e-5, 1, 4, 64, None) == (
+            "add_rms_norm: y must not be h, nor x or residual where it is of 8 bits")
+    for y, x, residual in ((FAKE, FAKE, other), (FAKE, other, FAKE)):
+        assert refused("int4gemv_add_rms_norm_quant", y, FAKE * 3, FAKE * 4, x, residual, FAKE * 5, 1e-5, 1,
+                       4, 64, None) == (
+            "add_rms_norm_quant: y must not be h, nor x or residual where it is of 8 bits")
+    c = cache()
+    assert refused("int4gemv_paged_attention", FAKE, FAKE, ctypes.addressof(c), FAKE, FAKE, 1.0, None, None,
+                   0, 3, 4, 5, FAKE, 1 << 40, None) == "paged_attention: out must not be q"
+    for lens, new_table in ((other, FAKE * 4), (FAKE * 5, FAKE * 3)):
+        assert refused("int4gemv_paged_evict", FAKE, other, ctypes.addressof(c), FAKE * 3, lens,
+                       new_table, 16, 4, 3, 5, 1, None) == (
+            "paged_evict: new_lens must not be seq_lens, nor new_table block_table")
