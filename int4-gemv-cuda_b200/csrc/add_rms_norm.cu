@@ -254,9 +254,10 @@ __global__ void __launch_bounds__(most_threads(kWhole, kPer), kPer == 2 && !kWho
       if (c >= chunks) continue;
       if (kWhole || (c + 1) * E <= left) {
         // what a chunk holds of neighbouring rows (several, where they are shorter than a chunk) is
-        // read, and left out of the sum
-        nx[j] = ld_stream_v4(x + c * E);
-        if (kResidual) nr[j] = ld_stream_v4(residual + c * E);
+        // read, and left out of the sum; h may be x or residual, but no block writes what this one
+        // takes of a chunk
+        nx[j] = ld_once_v4(x + c * E);
+        if (kResidual) nr[j] = ld_once_v4(residual + c * E);
       } else {  // the tensors end inside of the last chunk
         Chunk<T> fx, fr;
 #pragma unroll

@@ -140,6 +140,17 @@ struct Divider {
   }
 };
 
+// 16 bytes that the kernel reads once, and may write later (so not by the read-only path), kept out
+// of L1.
+__device__ __forceinline__ uint4 ld_once_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // 16 bytes of shared memory by their address.
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;

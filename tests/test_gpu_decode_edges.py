@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import decode_reference as ref
-from int4gemv import ops
+from int4gemv import capi, ops
 from test_gpu_decode_ops import BF16, F16, F32, assert_within, gen, no_status_left, randn, same_bits  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -44,3 +44,29 @@ def test_norm_of_rows_shorter_than_a_chunk(rows, hidden, dtype):
     w = 1 + randn(g, hidden, dtype=dtype, std=0.2)
     for residual in (None, r):
         check_norm(x, w, residual)
+
+
+@pytest.mark.parametrize("rows,hidden,dtype", [(2500, 4096, BF16), (1500, 8191, F16), (900, 16383, F16)])
+def test_norm_in_place_over_many_rows(rows, hidden, dtype):
+    """h in the place of x or of the residual where a block has several rows, each read while the one
+    before it is written."""
+    g = gen(rows)
+    x, r = randn(g, rows, hidden, dtype=dtype), randn(g, rows, hidden, dtype=dtype, std=4.0)
+    w = 1 + randn(g, hidden, dtype=dtype, std=0.2)
+    code = {F16: capi.DTYPE_F16, BF16: capi.DTYPE_BF16}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    y, h = ops.add_rms_norm(x, w, 1e-5, r)
+    q, scales, _ = ops.add_rms_norm_quant(x, w, 1e-5, r)
+    for place in range(2):
+        for eight in (False, True):
+            pair = [x.clone(), r.clone()]
+            out, out_scales = torch.empty_like(q if eight else y), torch.empty_like(scales)
+            args = (pair[place].data_ptr(), pair[0].data_ptr(), pair[1].data_ptr(), w.data_ptr(), 1e-5, code,
+                    rows, hidden, stream)
+            if eight:
+                capi.call("int4gemv_add_rms_norm_quant", out.data_ptr(), out_scales.data_ptr(), *args)
+                assert same_bits(out, q) and same_bits(out_scales, scales)
+            else:
+                capi.call("int4gemv_add_rms_norm", out.data_ptr(), *args)
+                assert same_bits(out, y)
+            assert same_bits(pair[place], h) and same_bits(pair[1 - place], (x, r)[1 - place])
