@@ -247,12 +247,14 @@ __global__ void __launch_bounds__(most_threads(kWhole, kPer), kPer == 2 && !kWho
     const int64_t at = row * a.hidden - shift;  // of the first chunk
     const T* x = static_cast<const T*>(a.x) + at;
     const T* residual = static_cast<const T*>(a.residual) + at;
-    const int64_t left = static_cast<int64_t>(a.rows) * a.hidden - at;  // elements up to the tensors' end
+    // chunks up to the tensors' end; the last one may be cut
+    const int64_t left = (static_cast<int64_t>(a.rows) * a.hidden - at) / E;
+    const int inside = left < chunks ? static_cast<int>(left) : chunks;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int c = tid + j * blockDim.x;
       if (c >= chunks) continue;
-      if (kWhole || (c + 1) * E <= left) {
+      if (kWhole || c < inside) {
         // what a chunk holds of neighbouring rows (several, where they are shorter than a chunk) is
         // read, and left out of the sum; h may be x or residual, but no block writes what this one
         // takes of a chunk
