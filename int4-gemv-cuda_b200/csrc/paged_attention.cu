@@ -32,6 +32,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <mutex>
 
 #include "decode.cuh"
@@ -229,6 +230,10 @@ __device__ __forceinline__ uint32_t load_tile(const Plan& p, Rows& rows, uint32_
   return mask;
 }
 
+// What a row's sums are divided by, given their maximum and sum: where nothing counted they are 0, and
+// so is the result.
+__device__ __forceinline__ float divisor(float2 ml) { return ml.x == -INFINITY ? 1.0f : ml.y; }
+
 // A warp's queries and sums for an item.
 template <class T, int DP, int NT, class S>
 struct Sums {
@@ -236,6 +241,7 @@ struct Sums {
   float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
   float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the reference of all lanes (a maximum, at most kRise
                              // below the largest score), this lane's sum
+  bool any;                  // a position has counted
 
   __device__ __forceinline__ void load_q(const Plan& p, int b, int item) {
     const int dim = p.a.cache.dim, g = threadIdx.x % kWarp / 4, t2 = threadIdx.x % 4 * 2;
@@ -268,6 +274,7 @@ struct Sums {
       m[j][0] = m[j][1] = -INFINITY;
       l[j][0] = l[j][1] = 0.0f;
     }
+    any = false;
   }
 
   // Adds the 16 positions at `tile`. scores: where this warp's go (kWeights). `after_qk` is called
@@ -281,6 +288,7 @@ struct Sums {
     const uint32_t k_at = tile + ((lane & 7) + (lane >> 3 & 1) * 8) * S::kPitch + (lane >> 4) * 16;
     const uint32_t v_at =
         tile + ((lane & 7) + (lane >> 4) * 8) * S::kPitch + (lane >> 3 & 1) * 16 + S::kHalf;
+    any |= mask != 0;
     // S^T: positions g, g + 8 by heads t2, t2 + 1
     float s[NT][4] = {};
 #pragma unroll
@@ -378,7 +386,10 @@ struct Sums {
     }
   }
 
-  // By the block: the warps' sums together, into joined and ml[0]. Ends with a barrier.
+  // By the block: the warps' sums together, into joined and ml[0]. Ends with a barrier. A maximum of
+  // -inf then says that nothing counted (an empty item, or pages that are all outside of the cache),
+  // which gives zeros; where positions counted, but all scores are -inf, it is the lowest number, and
+  // the result 0 / 0.
   __device__ __forceinline__ void join(float (&joined)[S::kRows][DP], float2 (&ml)[S::kWarps][S::kRows]) {
     const int warp = threadIdx.x / kWarp, g = threadIdx.x % kWarp / 4, t2 = threadIdx.x % 4 * 2;
 #pragma unroll
@@ -388,6 +399,7 @@ struct Sums {
         l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 4);
         l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 8);
         l[i][j] += __shfl_xor_sync(0xffffffffu, l[i][j], 16);
+        if (any) m[i][j] = fmaxf(m[i][j], -FLT_MAX);
         if (g == 0) ml[warp][i * 8 + t2 + j] = make_float2(m[i][j], l[i][j]);
       }
     }
@@ -697,7 +709,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
       const int pairs = c.dim / 2;
       for (int i = tid; i < rows * pairs; i += kThreads) {
         const int row = i / pairs, d = i % pairs * 2;
-        const float l_row = sh.ml[0][row].y;
+        const float l_row = divisor(sh.ml[0][row]);
         *reinterpret_cast<uint32_t*>(out + row * c.dim + d) =
             pack2<T>(sh.joined[row][d] / l_row, sh.joined[row][d + 1] / l_row);
       }
@@ -842,12 +854,12 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
     }
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
-      // a part whose scores are all -inf is not scaled: its sums are 0, or NaN
+      // a part in which nothing counted is not scaled: its sums are 0
       ml[r].x = ml[r].x == -INFINITY ? 1.0f : exp2_fast(ml[r].x - m);
       l = fmaf(ml[r].y, ml[r].x, l);
     }
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) sh.share[tid][r] = ml[r].x / l;
+    for (int r = 0; r < kMaxCluster; ++r) sh.share[tid][r] = ml[r].x / divisor(make_float2(m, l));
     sh.row_lse[tid] = m + log2f(l);
   }
   __syncthreads();
@@ -914,7 +926,7 @@ struct Parts {
     }
     return make_float2(m, warp_sum(l));
   }
-  // Of a part whose scores are all -inf nothing is scaled (its sums are 0, or NaN).
+  // Of a part in which nothing counted nothing is scaled (its sums are 0).
   static __device__ __forceinline__ float factor(float m, float top) {
     return m == -INFINITY ? 1.0f : exp2_fast(m - top);
   }
@@ -998,12 +1010,13 @@ __device__ __forceinline__ void join_head(const Plan& p) {
       }
     }
   }
+  const float l = divisor(ml);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int d = (j * kWarp + lane) * 4;
     if (d < dim) {
-      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(v[j].x / ml.y, v[j].y / ml.y),
-                                                      pack2<T>(v[j].z / ml.y, v[j].w / ml.y));
+      *reinterpret_cast<uint2*>(out + d) =
+          make_uint2(pack2<T>(v[j].x / l, v[j].y / l), pack2<T>(v[j].z / l, v[j].w / l));
     }
   }
 }

@@ -6,7 +6,8 @@ import torch
 
 import decode_reference as ref
 from int4gemv import capi, ops
-from test_gpu_decode_ops import BF16, F16, F32, assert_within, gen, no_status_left, randn, same_bits  # noqa: F401
+from test_gpu_decode_ops import (BF16, F16, F32, Paged, assert_within, check_attention, gen,  # noqa: F401
+                                 no_status_left, randn, same_bits)
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,63 @@ def test_norm_in_place_over_many_rows(rows, hidden, dtype):
                 capi.call("int4gemv_add_rms_norm", out.data_ptr(), *args)
                 assert same_bits(out, y)
             assert same_bits(pair[place], h) and same_bits(pair[1 - place], (x, r)[1 - place])
+
+
+# Tables for the kernel of small calls and, wider, for the one for any call.
+WIDTHS = [24, 6000]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("group,dim", [(4, 64), (17, 128), (3, 256)])
+def test_attention_of_refused_pages_gives_zeros(group, dim, weights, width):
+    """Sequences whose pages are all outside of the cache, as in the padded slots of a captured batch:
+    zeros, and nothing written; the others as they are without those."""
+    c = Paged([1, 200, 0, 300, 40], 2, dim, 16, F16, seed=dim, width=width)
+    q = randn(c.g, 5, 2 * group, dim, dtype=F16)
+    k = randn(c.g, 5, 2, dim, dtype=F16)
+    good = Paged([1, 200, 0, 300, 40], 2, dim, 16, F16, seed=dim, width=width)
+    want = ops.paged_attention(q, good.k, good.v, good.table, good.seq_lens, 0.1, k, k,
+                               good.weights if weights else None)
+    table = c.table.clone()
+    table[0], table[3], table[4, 1:] = -1, c.k.shape[0], 10**6
+    before = c.k.clone(), c.v.clone(), c.weights.clone()
+    out = ops.paged_attention(q, c.k, c.v, table, c.seq_lens, 0.1, k, k, c.weights if weights else None)
+    assert capi.device_status() == capi.STATUS_BAD_PAGE
+    assert (out[0] == 0).all() and (out[3] == 0).all() and (out[2] == 0).all()
+    assert same_bits(out[1], want[1]) and out[4].isfinite().all()
+    for b in (0, 3):  # the pages that these had are as they were
+        pages, offs = ref.positions(c.table[b], c.lens[b], 16)
+        assert same_bits(c.k[pages, offs], before[0][pages, offs])
+        assert same_bits(c.v[pages, offs], before[1][pages, offs])
+        assert same_bits(c.weights[pages, :, offs], before[2][pages, :, offs])
+    empty = torch.empty(0, 16, 2, dim, dtype=F16, device="cuda")
+    none = torch.empty(0, 2, 16, device="cuda")
+    out = ops.paged_attention(q, empty, empty, c.table, c.seq_lens, 0.1, k, k, none if weights else None)
+    assert capi.device_status() == capi.STATUS_BAD_PAGE
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+def test_attention_of_scores_without_a_softmax(width):
+    """Scores that are all -inf, a NaN or +inf among them: no softmax, so NaN, as the formula gives it;
+    some of -inf count as 0."""
+    c = Paged([20, 300, 300, 300, 300], 1, 64, 16, BF16, seed=1, width=width)
+    q = torch.ones(5, 4, 64, dtype=BF16, device="cuda")
+    at = [ref.positions(c.table[b], c.lens[b], 16) for b in range(5)]
+    c.k[at[0]] = float("-inf")
+    c.k[at[1]] = float("-inf")
+    c.k[at[2][0][7], at[2][1][7]] = float("nan")
+    c.k[at[3][0][299], at[3][1][299]] = float("inf")
+    some = torch.arange(300) % 3 != 0
+    c.k[at[4][0][some], at[4][1][some]] = float("-inf")
+    out = ops.paged_attention(q, c.k, c.v, c.table, c.seq_lens, 0.125)
+    assert out[:4].isnan().all()
+    kept = ~some
+    v = c.v[at[4][0][kept], at[4][1][kept], 0].double()
+    s = c.k[at[4][0][kept], at[4][1][kept], 0].double().sum(-1) * 0.125
+    p = torch.softmax(s, 0)
+    # scores of up to 4: off by 64 / 16 + 2 additions at 2^-22 of 0.125 sum|k| <= 32, as in
+    # ref.attention, and the pair of 16-bit numbers
+    bound = (2 * (6 * 2.0**-22 * 32 + 2.0**-20) + 2.0**-16 + 530 * 2.0**-23) * (p @ v.abs()) + 2.0**-8 * (p @ v).abs()
+    assert_within(out[4], (p @ v).expand(4, 64), bound.expand(4, 64))
