@@ -338,7 +338,8 @@ struct Sums {
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
         top[i][j] = fmaxf(v, m[i][j]);
-        rises |= v > m[i][j] + kRise;
+        // the difference, which is exact where it matters: m + kRise rounds where scores are large
+        rises |= v - m[i][j] > kRise;
       }
     }
     if (__any_sync(0xffffffffu, rises)) {

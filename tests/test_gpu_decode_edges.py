@@ -131,3 +131,28 @@ def test_attention_of_scores_without_a_softmax(width):
     # ref.attention, and the pair of 16-bit numbers
     bound = (2 * (6 * 2.0**-22 * 32 + 2.0**-20) + 2.0**-16 + 530 * 2.0**-23) * (p @ v.abs()) + 2.0**-8 * (p @ v).abs()
     assert_within(out[4], (p @ v).expand(4, 64), bound.expand(4, 64))
+
+
+@pytest.mark.parametrize("batch,width", [(80, 24), (500, 6000)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_of_scores_whose_steps_are_wide(dtype, batch, width):
+    """Scores of 2^27 (in base 2), whose neighbours are 16 apart: those of a later tile above the first
+    one's by one step, and by less than the rise at which a warp takes a new reference plus a step."""
+    c = Paged([300] * batch, 1, 64, 16, dtype, seed=4, width=width)
+    c.k.zero_()
+    pages, offs = ref.positions(c.table[0], 300, 16)
+    for b in range(batch):
+        pages, offs = ref.positions(c.table[b], 300, 16)
+        c.k[pages, offs, 0, 0] = 2.0**15
+        c.k[pages, offs, 0, 1] = 16.0
+        c.k[pages[200:], offs[200:], 0, 1] = 32.0
+    q = torch.zeros(batch, 2, 64, dtype=dtype, device="cuda")
+    q[..., 0], q[..., 1] = 2.0**12, 1
+    out = ops.paged_attention(q, c.k, c.v, c.table, c.seq_lens, 0.6931472)  # ln 2
+    want, _, probs, _ = ref.attention(q, c.k, c.v, c.table, c.lens, 0.6931472)
+    # the 100 later positions share all but 2^-15, whatever the rounding of the scores (a step off)
+    # does to the rest
+    for b in range(batch):
+        pages, offs = ref.positions(c.table[b], 300, 16)
+        v = c.v[pages[200:], offs[200:], 0].double()
+        assert_within(out[b], v.mean(0).expand(2, 64), (ref.HALF[dtype] + 2.0**-12) * (v.abs().max() * 2).expand(2, 64))
