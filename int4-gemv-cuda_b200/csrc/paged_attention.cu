@@ -46,9 +46,17 @@ namespace cg = cooperative_groups;
 constexpr int kWarpTile = 16;  // positions a warp takes of a tile
 constexpr int kMaxCluster = 8;
 constexpr int kMaxDim = 256;
-// A warp rescales its sums when a score passes their reference by this much (log2), not at every new
-// maximum: the factors stay at most 2^8, far inside of either 16-bit type.
+// A warp rescales its sums when a score passes their last maximum by this much (log2), not at every new
+// maximum.
 constexpr float kRise = 8.0f;
+// The reference is taken this much below the maximum (log2), so that probabilities begin at 2^kLift. An
+// fp16 number has steps of 2^-24 at the least, so what the MMA gets of a probability is off by up to
+// 2^-25 there: 2^-32 of the largest one with 7, and 2^(kRise + kLift) still fits the type. bf16 has
+// fp32's range and needs none.
+template <class T>
+constexpr float kLift = 0.0f;
+template <>
+constexpr float kLift<half> = 7.0f;
 
 // What depends on the head dimension rounded up to DP and the heads of an item, 8 NT; kSmall: the
 // kernel for small calls.
@@ -239,8 +247,8 @@ template <class T, int DP, int NT, class S>
 struct Sums {
   uint32_t qf[DP / 16][NT][2];
   float o[DP / 16][NT][4];   // dims g, g + 8 of 16 by heads t2, t2 + 1 of 8
-  float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the reference of all lanes (a maximum, at most kRise
-                             // below the largest score), this lane's sum
+  float m[NT][2], l[NT][2];  // heads t2, t2 + 1: the reference of all lanes (a maximum less kLift,
+                             // at most kLift + kRise below the largest score), this lane's sum
   bool any;                  // a position has counted
 
   __device__ __forceinline__ void load_q(const Plan& p, int b, int item) {
@@ -337,9 +345,9 @@ struct Sums {
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        top[i][j] = fmaxf(v, m[i][j]);
+        top[i][j] = fmaxf(v - kLift<T>, m[i][j]);
         // the difference, which is exact where it matters: m + kRise rounds where scores are large
-        rises |= v - m[i][j] > kRise;
+        rises |= v - m[i][j] > kRise + kLift<T>;
       }
     }
     if (__any_sync(0xffffffffu, rises)) {

@@ -133,6 +133,26 @@ def test_attention_of_scores_without_a_softmax(width):
     assert_within(out[4], (p @ v).expand(4, 64), bound.expand(4, 64))
 
 
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_far_below_a_peak(dtype, width):
+    """One position takes nearly all of the probability and has a value of 0: the result is the sum of
+    probabilities of 2^-25 each, which one 16-bit format or the other does not hold beside 1."""
+    c = Paged([64, 100], 2, 64, 16, dtype, seed=3, width=width)
+    q = torch.zeros(2, 6, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 1
+    for b, n in enumerate(c.lens):
+        pages, offs = ref.positions(c.table[b], n, 16)
+        c.k[pages, offs], c.v[pages, offs] = 0, 1000
+        c.k[pages[5], offs[5]], c.v[pages[5], offs[5]] = 17.4, 0
+    out = ops.paged_attention(q, c.k, c.v, c.table, c.seq_lens, 1.0)
+    want, bound, _, _ = ref.attention(q, c.k, c.v, c.table, c.lens, 1.0)
+    # an fp16 probability is off by up to 2^-25, where the largest is at least 2^7
+    tail = torch.tensor(c.lens, device="cuda")[:, None, None] * 2.0**-32 * 1000
+    assert want.min() > 1e-3 and (tail < 0.02 * want).all()
+    assert_within(out, want, bound + tail)
+
+
 @pytest.mark.parametrize("batch,width", [(80, 24), (500, 6000)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attention_of_scores_whose_steps_are_wide(dtype, batch, width):
