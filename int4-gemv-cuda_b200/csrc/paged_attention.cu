@@ -32,6 +32,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <mutex>
 
@@ -1103,30 +1104,67 @@ auto with_shape(int dim, int group, F f) {
 
 int64_t aligned_up(int64_t n) { return (n + 255) / 256 * 256; }
 
+// Clusters of `size` blocks of the kernel for small calls that the current device runs at once. A
+// cluster's blocks share a group of SMs, so that is less than SMs / size: on B200 74, 33 and 15 of 2, 4
+// and 8 blocks.
+template <int DP, int NT>
+int clusters_at_once(int size) {
+  static std::atomic<int> known[64][kMaxCluster + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return sm_count() / size;
+  std::atomic<int>& count = known[dev & 63][size];
+  int n = count.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  // the type and the weights do not matter: shared memory leaves room for one block an SM
+  const auto kernel = paged_attention_small_kernel<half, DP, NT, false>;
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(Shape<DP, NT, true>::kThreads);
+  cfg.dynamicSmemBytes = sizeof(SmallSmem<DP, NT>);
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = size;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSmem<DP, NT>)) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    return sm_count() / size;
+  }
+  count.store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // Fills the plan's sizes and, with a workspace, its pointers; returns the workspace's bytes, or -1
 // where the sizes are out of range.
 int64_t make_plan(const PagedAttentionArgs& a, Plan* p) {
   p->a = a;
   p->group = a.hq / a.cache.hkv;
   int ctas = 1, small_tile = 1;
+  int (*at_once)(int) = nullptr;
   with_shape(a.cache.dim, p->group, [&]<int DP, int NT>() {
     p->rows = Shape<DP, NT, false>::kRows;
     p->tile = Shape<DP, NT, false>::kTile;
     ctas = kCtas<DP, NT>;
     small_tile = Shape<DP, NT, true>::kTile;
+    at_once = clusters_at_once<DP, NT>;
   });
   p->head_tiles = (p->group + p->rows - 1) / p->rows;
   const int64_t items = static_cast<int64_t>(a.cache.hkv) * p->head_tiles;
   const int64_t len = static_cast<int64_t>(a.max_blocks) * a.cache.block_size;
-  // A small call: clusters as large as there is room for at one block an SM and as every block has a
-  // tile, if that leaves no block more than kSmallTiles. The weights of a KV head need all its query
-  // heads in one item.
+  // A small call: clusters as large as SMs allow at one block each and as every block has a tile, if that
+  // leaves no block more than kSmallTiles. Clusters that do not all run at once, and so take a second
+  // wave, only where the smaller ones leave a block more than half of that (16 sequences, one KV head of
+  // 128 dims: of up to 2000 positions 14.5 us in clusters of 8, 12.5 in clusters of 4; of up to 4000 16.6
+  // and 18.8). The weights of a KV head need all its query heads in one item.
   const int64_t all_items = a.batch * items, small_tiles = (len + small_tile - 1) / small_tile;
   p->cluster = 0;
   if (all_items > 0 && all_items <= sm_count() && small_tiles > 0 &&
       (!a.cache.weights || p->head_tiles == 1)) {
     int cluster = 1;
-    while (cluster < kMaxCluster && all_items * cluster * 2 <= sm_count() && cluster < small_tiles) {
+    while (cluster < kMaxCluster && all_items * cluster * 2 <= sm_count() && cluster < small_tiles &&
+           (all_items <= at_once(cluster * 2) || small_tiles > kSmallTiles / 2 * cluster)) {
       cluster *= 2;
     }
     if (small_tiles <= static_cast<int64_t>(kSmallTiles) * cluster) {

@@ -1,6 +1,11 @@
 """The decode-step operators where they can go wrong: rows shorter than a chunk and more rows than a
 grid has blocks, a tensor given twice, pages that are all refused, scores far apart."""
 
+import os
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -176,3 +181,50 @@ def test_attention_of_scores_whose_steps_are_wide(dtype, batch, width):
         pages, offs = ref.positions(c.table[b], 300, 16)
         v = c.v[pages[200:], offs[200:], 0].double()
         assert_within(out[b], v.mean(0).expand(2, 64), (ref.HALF[dtype] + 2.0**-12) * (v.abs().max() * 2).expand(2, 64))
+
+
+@pytest.mark.parametrize("hkv,n", [(8, 1000), (3, 500), (8, 4000)])
+def test_attention_of_clusters_around_what_runs_at_once(hkv, n):
+    """One to five sequences: items on both sides of the number of clusters that run at once."""
+    for batch in range(1, 6):
+        check_attention(Paged([n - 7 * b for b in range(batch)], hkv, 128, 16, F16, seed=batch), 4 * hkv, F16,
+                        True, True)
+
+
+FIRST_CALL = """
+import torch
+from int4gemv import capi, ops
+d = dict(device="cuda")
+x, w = torch.randn(8, 512, **d).half(), torch.ones(512, **d).half()
+q, kv = torch.randn(2, 4, 64, **d).half(), torch.randn(20, 16, 2, 64, **d).half()
+v = kv.clone()
+table = torch.arange(8, **d).int().view(2, 4)
+new = torch.arange(8, 16, **d).int().view(2, 4)
+lens = torch.tensor([60, 33], **d).int()
+weights = torch.rand(20, 2, 16, **d)
+tokens = torch.zeros(8, dtype=torch.int64, **d)
+
+def calls():
+    out = list(ops.add_rms_norm(x, w, 1e-5, x)) + list(ops.add_rms_norm_quant(x, w))
+    out += [ops.paged_attention(q, kv, v, table, lens, 0.125), ops.paged_attention(q, kv, v, table, lens, 0.1)]
+    out += ops.paged_evict(kv, v, weights, table, lens, new, 20, 5)
+    out += list(ops.token_logprobs(x, tokens, 3)) + list(ops.token_logprobs(x, tokens, 0))
+    return out
+
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = calls()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, calls()))
+assert capi.device_status() == 0
+print("captured first")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Kernels are loaded and their limits set on first use, which a capture has to allow."""
+    env = dict(os.environ, PYTHONPATH=str(Path(ops.LIBRARY_PATH).parents[1]))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL], env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured first" in run.stdout, run.stderr[-2000:]
