@@ -450,10 +450,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) token_logprobs_kernel(const L
     Sums sums = Sums::none();
     if constexpr (kTop) {
       if (tid == 0) sh.listed = sh.picked = sh.keyed = 0;
-      if (r.c0 >= r.c1) {  // a block without elements: no tile sets the maxima
-        if (tid < kGroups) sh.group_max[tid] = 0;
-        __syncthreads();
-      }
     }
 
     int tile = 0;
@@ -675,9 +671,9 @@ template <class T>
 cudaError_t launch(const LogprobArgs& a, cudaStream_t stream) {
   const int64_t chunks = (static_cast<int64_t>(a.vocab) + 2 * Chunk<T>::kElems) / Chunk<T>::kElems;
   const int room = kCtas * sm_count();
-  // A row is split as long as every thread keeps a chunk and there are at most two blocks an SM:
-  // what follows a row's stream costs a block as much as several tiles (64 rows of 128256 with 20
-  // alternatives: 16.5 us in clusters of 4, 23.7 in clusters of 8).
+  // A row is split as long as every thread keeps about a chunk (so no block is without one) and there
+  // are at most two blocks an SM: what follows a row's stream costs a block as much as several tiles (64
+  // rows of 128256 with 20 alternatives: 16.5 us in clusters of 4, 23.7 in clusters of 8).
   int cluster = 1;
   while (cluster < kMaxCluster && static_cast<int64_t>(a.rows) * cluster <= sm_count() &&
          chunks > static_cast<int64_t>(cluster) * kThreads) {
