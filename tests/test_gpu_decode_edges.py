@@ -11,8 +11,8 @@ import torch
 
 import decode_reference as ref
 from int4gemv import capi, ops
-from test_gpu_decode_ops import (BF16, F16, F32, Paged, assert_within, check_attention, gen,  # noqa: F401
-                                 no_status_left, randn, same_bits)
+from test_gpu_decode_ops import (BF16, F16, F32, Paged, assert_within, check_attention,  # noqa: F401
+                                 check_logprobs, gen, no_status_left, randn, same_bits)
 
 pytestmark = pytest.mark.gpu
 
@@ -228,3 +228,46 @@ def test_the_first_call_of_a_process_may_be_captured():
     env = dict(os.environ, PYTHONPATH=str(Path(ops.LIBRARY_PATH).parents[1]))
     run = subprocess.run([sys.executable, "-c", FIRST_CALL], env=env, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "captured first" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows,hidden,dtype", [
+    (1000, 4096, F16), (10000, 129, BF16), (6000, 64, F32), (20000, 7, F16),  # a chunk a thread, or one lane's
+    (1000, 8192, BF16), (1000, 8191, F16), (900, 8192, F32), (2000, 2049, F32),  # two
+    (700, 16383, F16), (600, 8301, F32),  # three
+    (450, 16384, BF16), (400, 20000, F16)])  # two in whole rows, and the loop that reads a row twice
+def test_norm_of_more_rows_than_blocks(rows, hidden, dtype):
+    """Blocks of several rows: the next one is read while one is stored, rows that end inside 16 bytes,
+    the tensors' end inside of the last ones."""
+    g = gen(rows + hidden)
+    x, w = randn(g, rows, hidden, dtype=dtype), 1 + randn(g, hidden, dtype=dtype, std=0.2)
+    r = randn(g, rows, hidden, dtype=dtype, std=4.0)
+    x[::7] *= 16  # rows of other sizes, whose statistics must not reach their neighbours
+    for residual in (None, r):
+        check_norm(x, w, residual)
+
+
+def test_norm_writes_h_without_a_residual():
+    """Through the C ABI h may be asked for without a residual: a copy of x, or x in its own place."""
+    g = gen(2)
+    x, w = randn(g, 300, 4096, dtype=BF16), randn(g, 4096, dtype=BF16)
+    want, _ = ops.add_rms_norm(x, w, 1e-5)
+    for h in (torch.empty_like(x), x):
+        y, before = torch.empty_like(x), x.clone()
+        capi.call("int4gemv_add_rms_norm", y.data_ptr(), h.data_ptr(), x.data_ptr(), None, w.data_ptr(), 1e-5,
+                  capi.DTYPE_BF16, 300, 4096, torch.cuda.current_stream().cuda_stream)
+        assert same_bits(h, before) and same_bits(x, before)
+        # the loop that reads a row twice adds its squares in another order
+        assert_within(y, want.double(), want.double().abs() * 2 * (ref.HALF[BF16] + ref.NORM_F32))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(1300, 5003, F16), (1300, 5003, F32), (1500, 1001, BF16),
+                                              (1200, 8192, F32), (700, 20000, F16)])
+def test_logprobs_of_more_rows_than_blocks(rows, vocab, dtype):
+    """Blocks of several rows, that begin at other places of 16 bytes, with and without alternatives."""
+    g = gen(vocab)
+    logits = randn(g, rows, vocab, dtype=dtype, std=3.0)
+    logits[::5] += 20  # other maxima, and a mask, from row to row
+    logits[::3, : vocab // 2] = float("-inf")
+    tokens = torch.randint(vocab, (rows,), generator=g, device="cuda")
+    for top in (0, 1, 7, 32):
+        check_logprobs(logits, tokens, top)
