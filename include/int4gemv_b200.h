@@ -309,7 +309,9 @@ int int4gemv_w4a16_exchange_static(void* y, const void* x, const void* qweight,
 
 /* Root-mean-square norm with the residual's addition. Per row of x [rows, hidden]:
  *   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight,
- * computed in fp32 from the unrounded sum; h and y are rounded once. x, residual, weight [hidden],
+ * computed in fp32 from the unrounded sum; h and y are rounded once. The squares are summed in fp32:
+ * a row whose sum passes 2^128 (fp32 or bf16 values of 1e19 / sqrt(hidden)) counts as infinite and gives
+ * y = 0; beside eps, squares below 2^-126 do not count. x, residual, weight [hidden],
  * h and y have one element type, dtype (INT4GEMV_DTYPE_F32, _F16 or _BF16). residual may be NULL (h = x);
  * h may then be NULL too, and is not written. h may be x or residual itself; y overlaps no other
  * tensor of the call. Any hidden >= 1; fastest when all pointers are 16-byte aligned. */
@@ -317,7 +319,7 @@ int int4gemv_add_rms_norm(void* y, void* h, const void* x, const void* residual,
                           float eps, int dtype, int64_t rows, int64_t hidden, void* stream);
 
 /* The same with y in 8 bits: scales[row] = max(max|y| / 448, 1e-12) (fp32), y = the e4m3 value
- * nearest to y / scales[row]. A row with a NaN or infinite sum has a NaN scale. */
+ * nearest to y / scales[row]. A row with a NaN or an infinity in h has a NaN scale. */
 int int4gemv_add_rms_norm_quant(void* y, float* scales, void* h, const void* x, const void* residual,
                                 const void* weight, float eps, int dtype, int64_t rows,
                                 int64_t hidden, void* stream);

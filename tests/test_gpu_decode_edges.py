@@ -271,3 +271,23 @@ def test_logprobs_of_more_rows_than_blocks(rows, vocab, dtype):
     tokens = torch.randint(vocab, (rows,), generator=g, device="cuda")
     for top in (0, 1, 7, 32):
         check_logprobs(logits, tokens, top)
+
+
+@pytest.mark.parametrize("rows,hidden", [(400, 4096), (1000, 1001), (3, 30000)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_of_values_whose_squares_pass_fp32(rows, hidden, dtype):
+    """Rows whose sum of squares passes 2^128 give y = 0 and the least scale, those with an infinity NaN;
+    h is right all the same, and so are the rows around them."""
+    g = gen(rows * hidden)
+    x, w = randn(g, rows, hidden, dtype=dtype), 1 + randn(g, hidden, dtype=dtype, std=0.2)
+    r = randn(g, rows, hidden, dtype=dtype, std=4.0)
+    x[::3, 5] = 1e20
+    x[1::3, 6] = float("inf")
+    y, h = ops.add_rms_norm(x, w, 1e-5, r)
+    q, scales, h2 = ops.add_rms_norm_quant(x, w, 1e-5, r)
+    assert same_bits(h, (x.double() + r.double()).to(dtype)) and same_bits(h, h2)
+    assert (y[::3] == 0).all() and (q[::3].float() == 0).all() and (scales[::3] == 1e-12).all()
+    assert scales[1::3].isnan().all() and y[1::3, 6].isnan().all()
+    # a call of fewer rows may sum a row by more threads, in another order: compared with 64 bits
+    want, _ = ref.norm(x[2::3], w, 1e-5, r[2::3])
+    assert_within(y[2::3], want, want.abs() * (ref.HALF[dtype] + ref.NORM_F32))
