@@ -12,7 +12,7 @@ import torch
 import decode_reference as ref
 from int4gemv import capi, ops
 from test_gpu_decode_ops import (BF16, F16, F32, Paged, assert_within, check_attention,  # noqa: F401
-                                 check_logprobs, gen, no_status_left, randn, same_bits)
+                                 check_evict, check_logprobs, gen, no_status_left, randn, same_bits)
 
 pytestmark = pytest.mark.gpu
 
@@ -291,3 +291,39 @@ def test_norm_of_values_whose_squares_pass_fp32(rows, hidden, dtype):
     # a call of fewer rows may sum a row by more threads, in another order: compared with 64 bits
     want, _ = ref.norm(x[2::3], w, 1e-5, r[2::3])
     assert_within(y[2::3], want, want.abs() * (ref.HALF[dtype] + ref.NORM_F32))
+
+
+# ---- Offsets behind 2^31 elements ----------------------------------------------------------------
+
+
+def test_norm_of_far_rows():
+    """Rows of a tensor of more than 2^31 elements, whole and odd."""
+    for hidden, rows in ((8192, 2**18 + 300), (8191, 2**18 + 300)):
+        x = torch.zeros(rows, hidden, dtype=BF16, device="cuda")
+        g = gen(hidden)
+        at = torch.tensor([0, 1, rows // 2, rows - 300, rows - 2, rows - 1], device="cuda")
+        x[at] = randn(g, 6, hidden, dtype=BF16)
+        w = 1 + randn(g, hidden, dtype=BF16, std=0.2)
+        assert x.numel() > 2**31
+        want, _ = ref.norm(x[at], w, 1e-5)
+        y, _ = ops.add_rms_norm(x, w)
+        assert_within(y[at], want, want.abs() * (ref.HALF[BF16] + ref.NORM_F32))
+        assert not y[rows - 3].any()
+
+
+def test_evict_of_far_pages():
+    """Old and new pages whose elements lie behind 2^31 elements."""
+    per_page = 16 * 2 * 128
+    c = Paged([300, 90], 2, 128, 16, F16, seed=6, spare=40, first_page=2**31 // per_page + 5)
+    assert c.k.stride(0) * c.table.max().item() > 2**31
+    check_evict(c, 100, 30)
+
+
+def test_logprobs_of_far_rows():
+    """Rows that lie 2^30 elements apart."""
+    flat = torch.empty(3 * 2**30 + 6000, dtype=F16, device="cuda")
+    logits = flat.as_strided((4, 5000), (2**30 + 1, 1))
+    g = gen(7)
+    for i in range(4):
+        logits[i] = randn(g, 5000, dtype=F16, std=3.0)
+    check_logprobs(logits, torch.tensor([0, 4999, 17, 2500], device="cuda"), 6)
