@@ -1130,6 +1130,7 @@ int clusters_at_once(int size) {
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallSmem<DP, NT>)) !=
           cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();  // not the next launch's
     return sm_count() / size;
   }
   count.store(n, std::memory_order_relaxed);
