@@ -350,16 +350,16 @@ size_t int4gemv_paged_cache_struct_bytes(void);
  * head h / (q_heads / kv_heads); q and out have the cache's type, the softmax and the sums are fp32.
  * q, out, k_new and v_new are 16-byte aligned, and out does not overlap q.
  * A sequence of length 0 gives zeros. block_table [batch, max_blocks] and seq_lens [batch] are
- * int32; table entries behind a sequence's last page are not read.
+ * int32; table entries behind a sequence's last page may be read, but are not used.
  * k_new, v_new ([batch, kv_heads, head_dim], or both NULL): the new token's key and value. seq_lens
  * counts that token; they are written to the slot of position seq_lens[b] - 1 and used for it.
  * That slot must not belong to another sequence of the batch.
  * add_weights: weights[page, g, offset] += the sum of the probabilities of the query heads of KV
  * head g, at every position; with k_new the new token's slot is set, not added to. Sequences of
- * one batch that share a page must then be given in different calls.
- * A length outside of [0, max_blocks block_size] is clamped, a page outside of [0, num_blocks) is
- * left out, and int4gemv_device_status reports 4; nothing outside of the cache is touched. A
- * sequence that has none of its pages gives zeros too.
+ * one batch that share a page must then be given in different calls, and a sequence names a page once.
+ * A length outside of [0, max_blocks block_size] is clamped (a new token beyond the table takes its last
+ * position), a page outside of [0, num_blocks) is left out, and int4gemv_device_status reports 4;
+ * nothing outside of the cache is touched. A sequence that has none of its pages gives zeros too.
  * workspace: int4gemv_paged_attention_workspace_size bytes on the device, 256-byte aligned, used
  * within the call in stream order (calls that may overlap need one each); its content does not
  * matter. The result does not depend on timing. */
@@ -370,7 +370,11 @@ int int4gemv_paged_attention(void* out, const void* q, const int4gemv_paged_cach
                              int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace for the current device (0 where none is needed), or -1 if the sizes are refused (see
- * int4gemv_last_error). The pointers of `cache` are not used. */
+ * int4gemv_last_error). The pointers of `cache` are not used. Without weights at most about 5 MB and 4
+ * bytes a sequence. With weights the scores are kept, 4 bytes for each sequence, position of the table
+ * (rounded up to tiles of 64 to 128) and query head (of a KV head an even number of them, or whole blocks
+ * of 16, 8 above 128 dims), whatever the lengths are: max_blocks should be what the longest sequence
+ * needs. */
 int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* cache, int64_t batch,
                                                 int64_t q_heads, int64_t max_blocks, int weights);
 
@@ -381,9 +385,10 @@ int64_t int4gemv_paged_attention_workspace_size(const int4gemv_paged_cache_t* ca
  * positions 0, 1, ... of the pages in new_table [batch, new_blocks]; new_lens [batch] =
  * min(n, budget); kept [batch, kv_heads, budget] holds the old positions, then -1. Heads choose
  * for themselves: afterwards position j of two heads may come from different tokens. The new pages
- * must not be among the old ones, nor be named twice, and new_lens and kept overlap no input; the
- * old pages are left as they were, so sequences may share them. Lengths and pages outside of the cache are treated as in
- * int4gemv_paged_attention (an unreadable weight counts as lowest, an unreadable page is not copied). */
+ * must not be among the old ones, nor be named twice, and new_lens and kept overlap no input; the old
+ * pages are left as they were, so sequences may share them. Lengths and pages outside of the cache are
+ * treated as in int4gemv_paged_attention (an unreadable weight counts as lowest, an unreadable page is not
+ * copied). The table has room for at most 2^31 - 8193 positions, and the budget is no larger. */
 int int4gemv_paged_evict(int32_t* kept, int32_t* new_lens, const int4gemv_paged_cache_t* cache,
                          const int32_t* block_table, const int32_t* seq_lens,
                          const int32_t* new_table, int64_t budget, int64_t recent, int64_t batch,

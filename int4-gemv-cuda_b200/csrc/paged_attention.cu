@@ -5,11 +5,13 @@
 // position's attention weight, summed over the query heads of its KV head, to a buffer that
 // eviction goes by.
 //
-// Bound by HBM: the cache is read once, 4 hq / hkv operations an element. Measured on B200 (fp16, 128
-// dims, 64 query and 8 KV heads): one sequence of 131072 positions 99 us, 5.4 TB/s (0.83 of a plain
-// copy's 6.53); 64 sequences of 512 to 8192 202 us (0.83). Of what is missing, 7 to 10 us are the scan
-// of the lengths, the first loads and the second kernel. Weights cost 7 us more at 24 sequences of up to
-// 4096 (48 to 55 us). Small calls are bound by latency: 701 positions of 32 query heads 7.5 us.
+// Bound by HBM and by the latency of a warp's chain of instructions: the cache is read once, 4 hq / hkv
+// operations an element. Measured on B200 (fp16, 128 dims, 64 query and 8 KV heads): one sequence of
+// 131072 positions 98 us, 5.5 TB/s (0.84 of a plain copy's 6.53); 64 sequences of 512 to 8192 194 us
+// (0.86). Of what is missing, 7 to 10 us are the scan of the lengths, the first loads and the second
+// kernel; in the rest the issue slots are a third busy, the tensor pipe an eighth, and three warps a
+// scheduler wait for their own results and copies. Weights cost 7 us more at 24 sequences of up to 4096
+// (48 to 55 us). Small calls are bound by latency alone: 701 positions of 32 query heads 7.6 us.
 //
 // Work: an item is (sequence, KV head, block of 8 or 16 query heads), cut into tiles of positions.
 // All tiles in order are split evenly over the blocks of the grid whatever the lengths are, so a
@@ -26,7 +28,8 @@
 // accumulators. The warp MMAs have the positions and the dimensions as rows and 8 query heads as
 // columns: S^T = K Q^T, O^T = V^T P^T, so a group of 8 heads or fewer fills half of what heads as
 // rows would take (P^T gets from the first product's layout to the second's by movmatrix). P is
-// given to the MMA as a sum of two 16-bit numbers, so its rounding does not show in the result.
+// given to the MMA as a sum of two 16-bit numbers, so its rounding does not show in the result (in fp16
+// what lies far below the largest is another matter, see kLift).
 // Positions behind the end are zero-filled in shared memory and masked, so nothing there reaches
 // a sum.
 #include <cooperative_groups.h>

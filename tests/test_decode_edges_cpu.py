@@ -4,6 +4,8 @@ import ctypes
 
 import pytest
 
+from int4gemv import capi
+
 from test_decode_ops_cpu import FAKE, cache, refused
 
 
@@ -37,3 +39,16 @@ def test_the_same_tensor_twice_is_refused():
         assert refused("int4gemv_paged_evict", FAKE, other, ctypes.addressof(c), FAKE * 3, lens,
                        new_table, 16, 4, 3, 5, 1, None) == (
             "paged_evict: new_lens must not be seq_lens, nor new_table block_table")
+
+
+@pytest.mark.parametrize("head_dim,group,counted", [(64, 4, 4), (128, 5, 6), (128, 16, 16), (64, 17, 32), (256, 3, 4),
+                                                    (192, 9, 16)])
+def test_workspace_of_weights_is_what_the_header_says(head_dim, group, counted):
+    """4 bytes a sequence, position of the table and counted query head, beside what a call without takes."""
+    size = capi.lib().int4gemv_paged_attention_workspace_size
+    for batch, blocks in ((3, 24), (40, 240)):  # 384 and 3840 positions, whole tiles of any kernel
+        a = ctypes.addressof(c := cache(head_dim=head_dim))
+        plain = size(a, batch, 2 * group, blocks, 0)
+        scores = 4 * batch * c.kv_heads * blocks * 16 * counted
+        assert 0 <= plain < 6 << 20
+        assert scores <= size(a, batch, 2 * group, blocks, 1) < scores + (6 << 20)
