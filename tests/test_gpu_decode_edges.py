@@ -293,6 +293,62 @@ def test_norm_of_values_whose_squares_pass_fp32(rows, hidden, dtype):
     assert_within(y[2::3], want, want.abs() * (ref.HALF[dtype] + ref.NORM_F32))
 
 
+@pytest.mark.parametrize("width", WIDTHS)
+def test_captured_attention_follows_its_inputs(width):
+    """One graph, replayed over lengths from nothing to the whole table, with pages, queries and new
+    tokens of each: what a decode loop does."""
+    c = Paged([300, 300, 300], 2, 128, 16, F16, seed=8, width=width)
+    q, k = randn(c.g, 3, 8, 128, dtype=F16), randn(c.g, 3, 2, 128, dtype=F16)
+    args = (q, c.k, c.v, c.table, c.seq_lens, 0.09, k, k, c.weights)
+    ops.paged_attention(*args)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.paged_attention(*args)
+    for lens in ((0, 0, 0), (1, 0, 300), (16, 17, 1), (128, 129, 255), (300, 64, 5)):
+        c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(randn(c.g, 3, 8, 128, dtype=F16))
+        k.copy_(randn(c.g, 3, 2, 128, dtype=F16))
+        c.table.copy_(c.table.roll(1, 0))
+        before = c.k.clone(), c.v.clone(), c.weights.clone()
+        g.replay()
+        after = out.clone(), c.k.clone(), c.v.clone(), c.weights.clone()
+        for t, was in zip((c.k, c.v, c.weights), before):
+            t.copy_(was)
+        want = ops.paged_attention(*args)
+        assert all(same_bits(a, b) for a, b in zip(after, (want, c.k, c.v, c.weights)))
+        assert all((out[b] == 0).all() for b in range(3) if lens[b] == 0)
+
+
+@pytest.mark.parametrize("k_layout,v_layout", [("heads", "tokens"), ("tokens", "pairs")])
+def test_caches_of_two_layouts(k_layout, v_layout):
+    """Keys and values with strides of their own."""
+    for width in WIDTHS:
+        c = Paged([200, 77, 0, 31], 3, 64, 16, BF16, seed=2, layout=k_layout, width=width, spare=60)
+        other = Paged([200, 77, 0, 31], 3, 64, 16, BF16, seed=2, layout=v_layout, width=width, spare=60)
+        c.v = other.v
+        assert c.k.stride() != c.v.stride()
+        check_attention(c, 12, BF16, True, True)
+        check_evict(c, 50, 9)
+
+
+def test_pages_longer_than_sequences():
+    """A contiguous cache: one page a sequence, of a size that is no power of two."""
+    c = Paged([5000, 1, 3777], 2, 64, 5003, F16, seed=3, spare=3)
+    check_attention(c, 10, F16, True, True)
+    check_evict(c, 2500, 100)
+
+
+def test_weights_that_are_not_aligned_to_four():
+    """Weights whose first element is no multiple of 16 bytes, in pages of a multiple of four."""
+    c = Paged([300, 90], 2, 64, 16, F16, seed=6, spare=40)
+    flat = torch.empty(c.weights.numel() + 1, device="cuda")
+    flat[1:] = c.weights.flatten()
+    c.weights = flat[1:].view_as(c.weights)
+    assert c.weights.data_ptr() % 16 == 4
+    check_attention(c, 8, F16, True, True)
+    check_evict(c, 100, 30)
+
+
 # ---- Offsets behind 2^31 elements ----------------------------------------------------------------
 
 
