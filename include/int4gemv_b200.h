@@ -357,9 +357,9 @@ size_t int4gemv_paged_cache_struct_bytes(void);
  * add_weights: weights[page, g, offset] += the sum of the probabilities of the query heads of KV
  * head g, at every position; with k_new the new token's slot is set, not added to. Sequences of
  * one batch that share a page must then be given in different calls, and a sequence names a page once.
- * A length outside of [0, max_blocks block_size] is clamped (a new token beyond the table takes its last
- * position), a page outside of [0, num_blocks) is left out, and int4gemv_device_status reports 4;
- * nothing outside of the cache is touched. A sequence that has none of its pages gives zeros too.
+ * A length outside of [0, max_blocks block_size] is clamped (a new token beyond the table is left out), a
+ * page outside of [0, num_blocks) is left out, and int4gemv_device_status reports 4; nothing outside of
+ * the cache is touched. A sequence that has none of its pages gives zeros too.
  * workspace: int4gemv_paged_attention_workspace_size bytes on the device, 256-byte aligned, used
  * within the call in stream order (calls that may overlap need one each); its content does not
  * matter. The result does not depend on timing. */

@@ -109,7 +109,11 @@ struct Plan {
 };
 
 __device__ __forceinline__ int clamped(const Plan& p, int n) { return min(max(n, 0), p.max_len); }
-__device__ __forceinline__ int length_of(const Plan& p, int b) { return clamped(p, p.a.lens[b]); }
+// The position of the new token of a sequence of the given length; -1 where the call brings none or the
+// table has no room for it (the last position there is another token's).
+__device__ __forceinline__ int new_position(const Plan& p, int given) {
+  return p.a.k_new && given <= p.max_len ? given - 1 : -1;
+}
 
 // The even split of `total` tiles: block c takes [start(c), start(c + 1)).
 struct Split {
@@ -165,11 +169,11 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t
 using Rows = const void* [kWarpTile][2];
 
 // By a warp, lanes 0-15 a position each: looks up the rows of 16 positions of sequence b from `pos`
-// (this lane's) on, given this lane's page, writes the new token's row where it is among them, and
-// starts the copies of K and V to `dst`. Returns the mask of positions that count.
+// (this lane's) on, given this lane's page, writes the new token's row where its position `fresh` is among
+// them, and starts the copies of K and V to `dst`. Returns the mask of positions that count.
 template <class T, class S>
 __device__ __forceinline__ uint32_t load_tile(const Plan& p, Rows& rows, uint32_t dst, int b, int n,
-                                              int item, int pos, int page) {
+                                              int fresh_at, int item, int pos, int page) {
   const PagedAttentionArgs& a = p.a;
   const PagedCache& c = a.cache;
   const int lane = threadIdx.x % kWarp;
@@ -182,7 +186,7 @@ __device__ __forceinline__ uint32_t load_tile(const Plan& p, Rows& rows, uint32_
       if (static_cast<unsigned>(page) < static_cast<unsigned>(c.num_blocks)) {
         const int off = pos - p.page.quotient(pos) * p.page.by;
         valid = true;
-        append = a.k_new != nullptr && pos == n - 1;
+        append = pos == fresh_at;
         k = static_cast<const T*>(c.k) + page * c.k_block + off * c.k_token + kv * c.k_head;
         v = static_cast<const T*>(c.v) + page * c.v_block + off * c.v_token + kv * c.v_head;
       } else {
@@ -467,13 +471,13 @@ struct Sums {
   }
 };
 
-// By a block of kThreads: adds the weights of `positions` positions of KV head kv of sequence b (n
-// long), from tile `tile0` of the sequence on, whose scores begin at tile `scores_tile`, for one item
-// (block `ht` of the head's query heads) whose rows have the sums row_lse. `ready` (by all threads, if
+// By a block of kThreads: adds the weights of `positions` positions of KV head kv of sequence b (whose
+// new token is at `fresh`), from tile `tile0` of the sequence on, whose scores begin at tile `scores_tile`,
+// for one item (block `ht` of the head's query heads) whose rows have the sums row_lse. `ready` (by all threads, if
 // there are positions) sees to those while the first loads are on their way.
 template <int kThreads, class F>
 __device__ __forceinline__ void add_weights(const Plan& p, int b, int kv, int ht, int rows,
-                                            int scores_tile, int tile0, int positions, int n,
+                                            int scores_tile, int tile0, int positions, int fresh,
                                             const float* row_lse, F ready) {
   constexpr int kAtOnce = 2, kFirst = 2;  // positions of a thread; pairs of rows loaded before `ready`
   const PagedAttentionArgs& a = p.a;
@@ -505,7 +509,7 @@ __device__ __forceinline__ void add_weights(const Plan& p, int b, int kv, int ht
       to[k] = c.weights + (static_cast<int64_t>(page[k]) * c.hkv + kv) * c.block_size +
               (pos - p.page.quotient(pos) * static_cast<int>(p.page.by));
       // a new token's slot may hold what its page was used for before
-      if (!(ht == 0 && a.k_new && pos == n - 1)) w[k] = *to[k];
+      if (!(ht == 0 && pos == fresh)) w[k] = *to[k];
     }
     if (i0 == 0) ready();
 #pragma unroll
@@ -535,12 +539,14 @@ __device__ __forceinline__ void add_weights(const Plan& p, int b, int kv, int ht
 
 // A position in the order of all tiles: sequence, item of the sequence, tile of the item.
 struct Walker {
-  int b, item, tile, tiles, n;
+  int b, item, tile, tiles, n, fresh;  // n: the length; fresh: the position of the new token, or -1
 
   template <int kTile>
   __device__ __forceinline__ void enter(const Plan& p) {  // to the next sequence with positions
     while (b < p.a.batch) {
-      n = length_of(p, b);
+      const int given = p.a.lens[b];
+      n = clamped(p, given);
+      fresh = new_position(p, given);
       if (n > 0) break;
       ++b;
     }
@@ -566,7 +572,7 @@ struct Smem {
   float joined[S::kRows][DP];
   float2 ml[S::kWarps][S::kRows];
   int scan[S::kWarps];
-  int start[3];  // sequence of the block's first tile, tiles before it, its length
+  int start[3];  // sequence of the block's first tile, tiles before it, its length as given
 };
 
 template <class T, int DP, int NT, bool kWeights>
@@ -584,7 +590,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
   const int tid = threadIdx.x, warp = tid / kWarp, lane = tid % kWarp;
 
   // Tiles before each sequence: a scan over the batch, a thread a sequence, in rounds. `find` is
-  // called with each thread's sequence, the tiles before and in it, and its length; returns the
+  // called with each thread's sequence, the tiles before and in it, and its length as given; returns the
   // tiles in all.
   auto scan = [&](auto find) {
     int before = 0;
@@ -608,15 +614,15 @@ __global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
         if (w < warp) t += sh.scan[w];
         sum += sh.scan[w];
       }
-      if (b < a.batch) find(b, before + t - own, own, n);
+      if (b < a.batch) find(b, before + t - own, own, given);
       before += sum;
       __syncthreads();  // sh.scan is written again
     }
     return before;
   };
   // a batch that fits one round keeps the scan's result in registers
-  int my_b = -1, my_before = 0, my_own = 0, my_n = 0;
-  const int total = scan([&](int b, int before, int own, int n) {
+  int my_b = -1, my_before = 0, my_own = 0, my_given = 0;
+  const int total = scan([&](int b, int before, int own, int given) {
     if (blockIdx.x == 0) {
       if (b == 0) p.first_tile[0] = 0;
       p.first_tile[b + 1] = before + own;
@@ -624,27 +630,28 @@ __global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
     my_b = b;
     my_before = before;
     my_own = own;
-    my_n = n;
+    my_given = given;
   });
   const Split split(total, p.blocks);
   const int t0 = split.start(blockIdx.x), t1 = split.start(blockIdx.x + 1);
   if (t0 >= t1) return;
-  auto is_start = [&](int b, int before, int own, int n) {
+  auto is_start = [&](int b, int before, int own, int given) {
     if (before <= t0 && t0 < before + own) {
       sh.start[0] = b;
       sh.start[1] = before;
-      sh.start[2] = n;
+      sh.start[2] = given;
     }
   };
   if (a.batch <= kThreads) {
-    if (my_b >= 0) is_start(my_b, my_before, my_own, my_n);
+    if (my_b >= 0) is_start(my_b, my_before, my_own, my_given);
     __syncthreads();
   } else {
     scan(is_start);
   }
   Walker load;
   load.b = sh.start[0];
-  load.n = sh.start[2];
+  load.n = clamped(p, sh.start[2]);
+  load.fresh = new_position(p, sh.start[2]);
   load.tiles = (load.n + kTile - 1) / kTile;
   load.item = (t0 - sh.start[1]) / load.tiles;
   load.tile = (t0 - sh.start[1]) % load.tiles;
@@ -665,7 +672,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, false>::kThreads, kCtas<DP, NT>)
     if (load_at < t1) {
       const uint32_t mask =
           load_tile<T, S>(p, sh.rows[warp], ring + load_stage * 2 * S::kHalf, load.b, load.n,
-                          load.item, position(), page);
+                          load.fresh, load.item, position(), page);
       if (lane == 0) sh.mask[warp][load_stage] = mask;
       load.next<kTile>(p);
       ++load_at;
@@ -791,7 +798,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
   Sums<T, DP, NT, S> sums;
   sums.load_q(p, b, item);
   sums.reset();
-  const int n = clamped(p, given);
+  const int n = clamped(p, given), fresh = new_position(p, given);
   if (given != n && tid == 0) atomicExch(p.status, kStatusBadPage);
   const int tiles = (n + kTile - 1) / kTile;
   const int own = tiles > rank ? (tiles - rank + ranks - 1) / ranks : 0;
@@ -802,7 +809,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
   auto load_next = [&] {
     if (loaded < own) {
       const uint32_t mask = load_tile<T, S>(
-          p, sh.rows[warp], ring + load_stage * 2 * S::kHalf, b, n, item,
+          p, sh.rows[warp], ring + load_stage * 2 * S::kHalf, b, n, fresh, item,
           (rank + loaded * ranks) * kTile + warp * kWarpTile + lane,
           sh.pages[warp][loaded][lane % kWarpTile]);
       if (lane == 0) sh.mask[warp][load_stage] = mask;
@@ -895,7 +902,7 @@ __global__ void __launch_bounds__(Shape<DP, NT, true>::kThreads)
     for (int i = 0; i < own; ++i) {
       const int tile = rank + i * ranks;
       add_weights<kThreads>(p, b, kv, 0, rows, index * p.item_tiles + tile, tile,
-                            min(kTile, n - tile * kTile), n, sh.row_lse, [] {});
+                            min(kTile, n - tile * kTile), fresh, sh.row_lse, [] {});
     }
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -1052,7 +1059,8 @@ __device__ __forceinline__ void join_weights(const Plan& p, int block, int block
   int b = start;
   while (t < t1) {
     while (p.first_tile[b + 1] / p.head_tiles <= t) ++b;
-    const int n = length_of(p, b), tiles = (n + p.tile - 1) / p.tile;
+    const int given = a.lens[b], n = clamped(p, given), fresh = new_position(p, given);
+    const int tiles = (n + p.tile - 1) / p.tile;
     const int first = p.first_tile[b] / p.head_tiles;
     const int kv = (t - first) / tiles, tile0 = (t - first) % tiles;
     const int count = min(tiles - tile0, t1 - t);
@@ -1061,7 +1069,7 @@ __device__ __forceinline__ void join_weights(const Plan& p, int block, int block
       const int rows = min(p.group - ht * p.rows, p.rows);
       const Parts parts(p, total, begin, tiles);
       add_weights<kJoinThreads>(
-          p, b, kv, ht, rows, begin + tile0, tile0, min(count * p.tile, n - tile0 * p.tile), n, row_lse,
+          p, b, kv, ht, rows, begin + tile0, tile0, min(count * p.tile, n - tile0 * p.tile), fresh, row_lse,
           [&] {
             if (parts.count == 1) {
               if (tid < rows) {

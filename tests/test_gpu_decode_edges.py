@@ -294,6 +294,37 @@ def test_norm_of_values_whose_squares_pass_fp32(rows, hidden, dtype):
 
 
 @pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("group", [4, 17])
+def test_attention_new_token_beyond_the_table(group, width):
+    """The table's last position belongs to an earlier token, which the new one must not replace: the call
+    is as without new tokens, and the status says so."""
+    page = 16
+    c = Paged([64, width * page, 100], 2, 64, page, F16, seed=9, width=width)
+    q, k = randn(c.g, 3, 2 * group, 64, dtype=F16), randn(c.g, 3, 2, 64, dtype=F16)
+    lens = c.seq_lens.clone()
+    lens[1] += 3
+    before = c.k.clone(), c.v.clone(), c.weights.clone()
+    want = ops.paged_attention(q[1:2], c.k, c.v, c.table[1:2], c.seq_lens[1:2], 0.1, weights=c.weights)
+    pages, offs = ref.positions(c.table[1], width * page, page)
+    want_w = c.weights[pages, :, offs]
+    for t, was in zip((c.k, c.v, c.weights), before):
+        t.copy_(was)
+    out = ops.paged_attention(q, c.k, c.v, c.table, lens, 0.1, k, k, c.weights)
+    assert capi.device_status() == capi.STATUS_BAD_PAGE
+    assert same_bits(c.k[pages, offs], before[0][pages, offs])
+    assert same_bits(c.v[pages, offs], before[1][pages, offs])
+    # another batch may split the sequence elsewhere: both are within the bound of the 64-bit result
+    _, bound, probs, rel = ref.attention(q, c.k, c.v, c.table, c.lens, 0.1)
+    assert_within(out[1:2], want.double(), 2 * bound[1:2])
+    p = probs[1].sum(1).T
+    bound_w = 2 * (p * (rel[1] + group * ref.F32) + (want_w.double() * 2 * ref.F32) + group * 2.0**-126)
+    assert_within(c.weights[pages, :, offs], want_w.double(), bound_w)
+    for b in (0, 2):  # the others got theirs
+        pages, offs = ref.positions(c.table[b], c.lens[b], page)
+        assert same_bits(c.k[pages[-1], offs[-1]], k[b])
+
+
+@pytest.mark.parametrize("width", WIDTHS)
 def test_captured_attention_follows_its_inputs(width):
     """One graph, replayed over lengths from nothing to the whole table, with pages, queries and new
     tokens of each: what a decode loop does."""
