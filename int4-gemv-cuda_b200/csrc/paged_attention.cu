@@ -8,10 +8,11 @@
 // Bound by HBM and by the latency of a warp's chain of instructions: the cache is read once, 4 hq / hkv
 // operations an element. Measured on B200 (fp16, 128 dims, 64 query and 8 KV heads): one sequence of
 // 131072 positions 98 us, 5.5 TB/s (0.84 of a plain copy's 6.53); 64 sequences of 512 to 8192 194 us
-// (0.86), 207 on another card. Of what is missing, 7 to 10 us are the scan of the lengths, the first loads and the second
-// kernel; in the rest the issue slots are a third busy, the tensor pipe an eighth, and three warps a
-// scheduler wait for their own results and copies. Weights cost 7 us more at 24 sequences of up to 4096
-// (48 to 55 us). Small calls are bound by latency alone: 701 positions of 32 query heads 7.6 us.
+// (0.86), 207 on another card. Of what is missing, 7 to 10 us are the scan of the lengths, the first
+// loads and the second kernel; in the rest the issue slots are a third busy, the tensor pipe an eighth,
+// and three warps a scheduler wait for their own results and copies. Weights cost 7 us more at 24
+// sequences of up to 4096 (48 to 55 us). Small calls are bound by latency alone: 701 positions of 32
+// query heads 7.6 us.
 //
 // Work: an item is (sequence, KV head, block of 8 or 16 query heads), cut into tiles of positions.
 // All tiles in order are split evenly over the blocks of the grid whatever the lengths are, so a
